@@ -305,6 +305,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdShape<DP>::ctas)
                         const float f = m == neg_inf() ? 0.0f : ex2(m - mn);
                         l *= f;
                         m = mn;
+                        wait_st();  // the half before may have stored P and a rescaled O: both are read back here
                         if (w > 0) {  // the other half's P, already written
                             uint32_t q[16];
                             tmem_ld16(ts, q);

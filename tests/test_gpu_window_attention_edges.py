@@ -1,0 +1,22 @@
+"""Windowed attention on the GPU where single rows go wrong: maxima that keep growing, rows and columns that
+hold what is not finite, rows that a bias masks throughout, extreme arguments."""
+
+import pytest
+import torch
+
+from .attention_ref import check, reference
+from .test_gpu_window_attention import DT, call, make, verify
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 72, 96, 128])
+@pytest.mark.parametrize("window,sinks", [((-1, -1), 0), ((-1, 0), 0), ((150, 40), 9)])
+def test_maxima_that_grow_all_along(dt, dim, window, sinks):
+    """Logits rise by 16 with every 32 keys, so that a row's reference of the exponents moves in each half of
+    every tile: what was written before (P of the other half, the output) is rescaled again and again."""
+    c = make(40, [300, 77], 2, 1, dim, DT[dt])
+    c["q"][..., 0] = dim ** 0.5
+    c["k"][..., 0] = torch.cat([torch.arange(300), torch.arange(77)]).cuda()[:, None] * 0.5
+    verify(c, window, sinks)
