@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                 fence_after();
                 if (pass > 0) {
                     const uint32_t tile = smem_addr(smem) + S::k + ring_k.at * S::tile_bytes;
-                    ok = mbar_wait(bar_k + 8 * ring_k.at, ring_k.parity);
+                    // the tile is changed under neither half's products: S of both has to be done
+                    ok = mbar_wait(bar_k + 8 * ring_k.at, ring_k.parity) && mbar_wait(bar_s + 8 * (half ^ 1), parity);
                     const uint2 bad = zero_nonfinite<S::panels>(tile, bad_rows, bar_fix, t_now.i, tid, ok);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
@@ -653,7 +654,9 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                 fence_after();
                 if (pass > 0) {
                     const uint32_t at = smem_addr(smem) + ring.at * S::tile_bytes;
-                    ok = mbar_wait(bar_q + 8 * ring.at, ring.parity) && mbar_wait(bar_d + 8 * ring.at, ring.parity);
+                    // the tiles are changed under neither half's products: S and dP of both have to be done
+                    ok = mbar_wait(bar_q + 8 * ring.at, ring.parity) && mbar_wait(bar_d + 8 * ring.at, ring.parity) &&
+                         mbar_wait(bar_s + 8 * (half ^ 1), parity);
                     const uint2 bq = zero_nonfinite<S::panels>(at + S::q, bad_rows[0], bar_fix, i, tid, ok);
                     const uint2 bd = zero_nonfinite<S::panels>(at + S::d, bad_rows[1], bar_fix + 8, i, tid, ok);
                     ok = __all_sync(0xffffffffu, ok);

@@ -20,3 +20,22 @@ def test_maxima_that_grow_all_along(dt, dim, window, sinks):
     c["q"][..., 0] = dim ** 0.5
     c["k"][..., 0] = torch.cat([torch.arange(300), torch.arange(77)]).cuda()[:, None] * 0.5
     verify(c, window, sinks)
+
+
+def test_bucket_sums_beside_keys_of_minus_infinity():
+    """Keys with a component of -inf where every query is positive have logits of -inf: weight 0. dQ of the rows
+    that see one is 0 times infinity, so the gradients' second pass runs; the bucket sums are those of the
+    other keys, the same bits each time."""
+    c = make(41, [700, 130], 2, 1, 64, torch.bfloat16, buckets=16)
+    c["q"][..., 0] = 1.0
+    at = torch.tensor([35, 45, 60, 63, 100, 127, 400, 700 + 50, 700 + 120])
+    c["k"][at.cuda(), :, 0] = -float("inf")
+    first = None
+    for _ in range(5):
+        got = call(c, (90, 70), 3)
+        want = reference(c["q"], c["k"], c["v"], c["ptr_q"].tolist(), c["ptr_k"].tolist(), 90, 70, 3, 0.125, c["bias"],
+                         c["pos_q"], c["pos_k"], 0.4, 4, c["dout"], True) if first is None else want
+        for n in ("out", "dk", "dv", "dbias"):
+            check(got[n], want[n], n)
+        first = got if first is None else first
+        assert torch.equal(got["dbias"], first["dbias"])
