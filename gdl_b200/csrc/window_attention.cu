@@ -38,7 +38,8 @@ int check(const gdl_attention *a) {
     GDL_RETURN_IF(a->n_key > 0 && (!a->k || !a->v), GDL_ERR_INVALID);
     if (a->bias) {
         GDL_RETURN_IF(a->buckets < 1 || a->buckets > kAttnMaxBuckets || a->steps_log2 < 0 || a->steps_log2 > 4 ||
-                          (a->bias_dtype != GDL_DTYPE_F32 && a->bias_dtype != GDL_DTYPE_BF16),
+                          (a->bias_dtype != GDL_DTYPE_F32 && a->bias_dtype != GDL_DTYPE_BF16) ||
+                          !(a->inv_radius2 >= 0.0f && a->inv_radius2 <= 3.4028234e38f),  // (t below 1 has no bucket)
                       GDL_ERR_INVALID);
         GDL_RETURN_IF((a->n_query > 0 && !a->pos_q) || (a->n_key > 0 && !a->pos_k), GDL_ERR_INVALID);
     }

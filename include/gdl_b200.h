@@ -452,7 +452,7 @@ typedef struct {
     float scale;
     const void *bias;                /* [heads, buckets] contiguous, nullable                         */
     int32_t bias_dtype, buckets, steps_log2; /* 1 <= buckets <= 64, 0 <= steps_log2 <= 4              */
-    float inv_radius2;
+    float inv_radius2;               /* finite, at least 0                                            */
     const float *pos_q, *pos_k;      /* [n_query, 3], [n_key, 3] f32; needed with a bias              */
     int32_t *status;                 /* nullable device word: GDL_ERR_TIMEOUT if a bounded wait of a
                                         kernel gave up (never observed; its rows are then NaN)        */
