@@ -31,18 +31,20 @@ def _spread(v: Tensor) -> Tensor:
 def morton_order(pos: Tensor, ptr: Tensor) -> Tensor:
     """[N] int64 permutation: each cloud's rows (clouds stay in place) by the 30-bit Morton code of their
     positions within the cloud's bounding cube; equal codes keep their order. Clouds are packed by ptr
-    [B + 1], which has to cover all rows."""
+    [B + 1]; rows of no cloud stay where they are."""
     n, clouds = pos.shape[0], ptr.numel() - 1
-    ptr = ptr.to(pos.device)
-    cloud = torch.repeat_interleave(torch.arange(clouds, device=pos.device), ptr[1:] - ptr[:-1], output_size=n)
+    ptr = ptr.to(pos.device, torch.int64)
+    # cloud + 1 of each row: 0 before the first cloud, clouds + 1 behind the last
+    at = torch.searchsorted(ptr, torch.arange(n, device=pos.device), right=True)
     p = pos.detach().float()
-    at = cloud[:, None].expand(-1, 3)
-    low = torch.full((clouds, 3), float("inf"), device=p.device).scatter_reduce_(0, at, p, "amin")
-    high = torch.full((clouds, 3), -float("inf"), device=p.device).scatter_reduce_(0, at, p, "amax")
+    rows = at[:, None].expand(-1, 3)
+    low = torch.full((clouds + 2, 3), float("inf"), device=p.device).scatter_reduce_(0, rows, p, "amin")
+    high = torch.full((clouds + 2, 3), -float("inf"), device=p.device).scatter_reduce_(0, rows, p, "amax")
     side = (high - low).amax(1).clamp(min=1e-30)
-    cell = ((p - low[cloud]) / side[cloud, None] * 1023.0).long().clamp_(0, 1023)
+    cell = ((p - low[at]) / side[at, None] * 1023.0).long().clamp_(0, 1023)
     code = _spread(cell[:, 0]) | (_spread(cell[:, 1]) << 1) | (_spread(cell[:, 2]) << 2)
-    return torch.argsort((cloud << 30) | code, stable=True)
+    code = torch.where((at > 0) & (at <= clouds), code, 0)
+    return torch.argsort((at << 30) | code, stable=True)
 
 
 class SerializedScan(nn.Module):

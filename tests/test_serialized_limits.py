@@ -2,6 +2,9 @@
 extreme arguments."""
 
 import pytest
+import torch
+
+from gdl_b200.serialized import morton_order
 
 from .test_serialized_host import INVALID, attention, lib  # noqa: F401
 
@@ -12,3 +15,18 @@ def test_a_bucket_scale_below_zero_or_not_finite_is_refused(lib, inv_radius2):  
     a = attention(bias=4096, buckets=8, pos_q=4096, pos_k=4096, inv_radius2=inv_radius2)
     assert lib.gdl_window_attention(a, 4096, None, None, None) == INVALID
     assert lib.gdl_window_attention_backward(a, 4096, 4096, None, 4096, 4096, 4096, 4096, 4096, 4096, 1 << 40, None) == INVALID
+
+
+def test_morton_order_leaves_rows_of_no_cloud_in_their_places():
+    """Bounds that do not cover all rows (the operators give such rows 0): an index made of them must stay in range."""
+    g = torch.Generator().manual_seed(0)
+    pos = torch.rand(100, 3, generator=g)
+    for bounds in ([10, 40, 40, 85], [0, 60], [30, 100], [50, 50], [0]):
+        order = morton_order(pos, torch.tensor(bounds))
+        assert torch.equal(order.sort()[0], torch.arange(100))
+        assert torch.equal(order[:bounds[0]], torch.arange(bounds[0]))
+        assert torch.equal(order[bounds[-1]:], torch.arange(bounds[-1], 100))
+        for s, e in zip(bounds[:-1], bounds[1:]):  # each cloud as if it were alone
+            assert torch.equal(order[s:e] - s, morton_order(pos[s:e], torch.tensor([0, e - s])))
+    assert morton_order(pos[:0], torch.tensor([0, 0])).shape == (0,)
+    assert torch.equal(morton_order(pos, torch.tensor([0, 30, 100], dtype=torch.int32)), morton_order(pos, torch.tensor([0, 30, 100])))
