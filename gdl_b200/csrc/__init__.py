@@ -587,7 +587,7 @@ def once_only(what: str) -> None:
 
 
 def _bounds(ptr: torch.Tensor, dev: torch.device) -> torch.Tensor:
-    if ptr.is_cuda and ptr.dtype == torch.int64 and ptr.is_contiguous():
+    if ptr.is_cuda and ptr.device == dev and ptr.dtype == torch.int64 and ptr.is_contiguous():
         return ptr
     return nat.to_device(ptr, dev, torch.int64)
 

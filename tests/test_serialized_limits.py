@@ -4,6 +4,7 @@ extreme arguments."""
 import pytest
 import torch
 
+from gdl_b200 import csrc
 from gdl_b200.serialized import morton_order
 
 from .test_serialized_host import INVALID, attention, lib  # noqa: F401
@@ -30,3 +31,17 @@ def test_morton_order_leaves_rows_of_no_cloud_in_their_places():
             assert torch.equal(order[s:e] - s, morton_order(pos[s:e], torch.tensor([0, e - s])))
     assert morton_order(pos[:0], torch.tensor([0, 0])).shape == (0,)
     assert torch.equal(morton_order(pos, torch.tensor([0, 30, 100], dtype=torch.int32)), morton_order(pos, torch.tensor([0, 30, 100])))
+
+
+def test_bounds_on_another_gpu_are_copied(monkeypatch):
+    """A kernel must not be given another GPU's memory: bounds pass as they are only on the rows' own device."""
+    class Bounds:
+        is_cuda, dtype, device = True, torch.int64, torch.device("cuda", 1)
+
+        def is_contiguous(self):
+            return True
+
+    monkeypatch.setattr(csrc.nat, "to_device", lambda t, dev, dtype: ("copied", dev))
+    there = Bounds()
+    assert csrc._bounds(there, torch.device("cuda", 0)) == ("copied", torch.device("cuda", 0))
+    assert csrc._bounds(there, torch.device("cuda", 1)) is there
