@@ -90,14 +90,12 @@ __device__ __forceinline__ void stage_row(float *s, const T *p, int dim) {
 
 // The logit (in powers of two) of global query row qi, staged in sq, and global key row kj, head h.
 template <typename T>
-__device__ __forceinline__ float logit2(const gdl_attention &a, int h, const float *sq, int64_t qi, int64_t kj,
-                                        int &bucket) {
+__device__ __forceinline__ float logit2(const gdl_attention &a, int h, const float *sq, int64_t qi, int64_t kj) {
     const T *kp = (const T *)a.k + kj * a.k_row + (int64_t)(h / (a.heads / a.kv_heads)) * a.k_head;
     float s = row_dot(sq, kp, a.dim) * (a.scale * kLog2e);
-    bucket = 0;
     if (a.bias) {
         const float *p = a.pos_q + 3 * qi, *r = a.pos_k + 3 * kj;
-        bucket = distance_bucket(a, p[0], p[1], p[2], r[0], r[1], r[2]);
+        const int bucket = distance_bucket(a, p[0], p[1], p[2], r[0], r[1], r[2]);
         s = fmaf(bias_at(a, (int64_t)h * a.buckets + bucket), kLog2e, s);
     }
     return s;
@@ -120,8 +118,7 @@ __device__ __noinline__ void attention_row(const gdl_attention &a, int h, int64_
         const int64_t from = part ? r.lo : 0, to = part ? r.hi : r.sinks;
         for (int64_t j0 = from; j0 < to; j0 += 32) {
             const int64_t j = j0 + lane;
-            int bucket;
-            const float s = j < to ? logit2<T>(a, h, sq, qi, k0 + j, bucket) : neg_inf();
+            const float s = j < to ? logit2<T>(a, h, sq, qi, k0 + j) : neg_inf();
             const float mn = fmaxf(m, warp_max(s));
             const float base = mn == neg_inf() ? 0.0f : mn;
             const float c = ex2(m - base);
@@ -148,12 +145,11 @@ __device__ __noinline__ void attention_row(const gdl_attention &a, int h, int64_
     if (lse && lane == 0) lse[(int64_t)h * a.n_query + qi] = l == 0.0f ? neg_inf() : (m + log2f(l)) * kLn2;
 }
 
-// One warp: dq of a query row. `hist` (nullable; two values a lane, bucket b in lane b % 32, value b / 32)
-// takes the row's sums of dS by bucket. sq, sd: strips of the warp's own. delta[h][qi] is written.
+// One warp: dq of a query row, delta known. sq, sd: strips of the warp's own.
 template <typename T>
 __device__ __noinline__ void attention_dq_row(const gdl_attention &a, int h, int64_t q0, int64_t nq, int64_t k0,
-                                              int64_t nk, int64_t row, float *sq, float *sd, const T *out,
-                                              const float *lse, const T *dout, T *dq, float *delta, float *hist) {
+                                              int64_t nk, int64_t row, float *sq, float *sd,
+                                              const float *lse, const float *delta, const T *dout, T *dq) {
     const int lane = threadIdx.x & 31;
     const int64_t qi = q0 + row;
     const int hk = h / (a.heads / a.kv_heads);
@@ -162,11 +158,7 @@ __device__ __noinline__ void attention_dq_row(const gdl_attention &a, int h, int
     stage_row(sq, (const T *)a.q + qi * a.q_row + (int64_t)h * a.q_head, a.dim);
     stage_row(sd, dout + ro, a.dim);
     __syncwarp();
-    float de = 0.0f;
-    for (int d = lane; d < a.dim; d += 32) de = fmaf(sd[d], load1(out + ro + d), de);
-    de = warp_sum(de);
-    if (lane == 0) delta[(int64_t)h * a.n_query + qi] = de;
-    const float ls = lse[(int64_t)h * a.n_query + qi];
+    const float de = delta[(int64_t)h * a.n_query + qi], ls = lse[(int64_t)h * a.n_query + qi];
     const KeyRange r = visible_keys(a, row + nk - nq, nk);
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (ls != neg_inf()) {
@@ -174,31 +166,26 @@ __device__ __noinline__ void attention_dq_row(const gdl_attention &a, int h, int
             const int64_t from = part ? r.lo : 0, to = part ? r.hi : r.sinks;
             for (int64_t j0 = from; j0 < to; j0 += 32) {
                 const int64_t j = j0 + lane;
-                int bucket = 0;
                 float ds = 0.0f;
                 if (j < to) {
-                    const float p = ex2(logit2<T>(a, h, sq, qi, k0 + j, bucket) - ls * kLog2e);
+                    const float p = ex2(logit2<T>(a, h, sq, qi, k0 + j) - ls * kLog2e);
                     const T *vp = (const T *)a.v + (k0 + j) * a.v_row + (int64_t)hk * a.v_head;
                     ds = p * (row_dot(sd, vp, a.dim) - de);
                 }
                 const int cnt = to - j0 < 32 ? (int)(to - j0) : 32;
                 for (int t = 0; t < cnt; ++t) {
                     const float dt = __shfl_sync(0xffffffffu, ds, t);
-                    const int bt = __shfl_sync(0xffffffffu, bucket, t);
                     const T *kp = (const T *)a.k + (k0 + j0 + t) * a.k_row + (int64_t)hk * a.k_head;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (lane + 32 * e < a.dim) acc[e] = fmaf(dt, load1(kp + lane + 32 * e), acc[e]);
-                    if (hist && (bt & 31) == lane) hist[bt >> 5] += dt;
                 }
             }
         }
     }
-    if (dq) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (lane + 32 * e < a.dim) store1(dq + ro + lane + 32 * e, acc[e] * a.scale);
-    }
+    for (int e = 0; e < 4; ++e)
+        if (lane + 32 * e < a.dim) store1(dq + ro + lane + 32 * e, acc[e] * a.scale);
 }
 
 // One warp: dk and dv of a key row, for one head of keys and values.

@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int r = warp; r < rows; r += kThreads / 32)
         if (again[r >> 5] >> (r & 31) & 1)
             attention_dq_row<T>(a, h, t.start, t.n, k0, nk, t.first + r, P + warp * 2 * kAttnMaxDim,
-                                P + (warp * 2 + 1) * kAttnMaxDim, out, lse, dout, dq, delta, nullptr);
+                                P + (warp * 2 + 1) * kAttnMaxDim, lse, delta, dout, dq);
     if (part)
         for (int b = warp; b < a.buckets; b += kThreads / 32) {
             float s = 0.0f;
