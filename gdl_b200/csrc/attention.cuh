@@ -188,11 +188,13 @@ __device__ __noinline__ void attention_dq_row(const gdl_attention &a, int h, int
         if (lane + 32 * e < a.dim) store1(dq + ro + lane + 32 * e, acc[e] * a.scale);
 }
 
-// One warp: dk and dv of a key row, for one head of keys and values.
+// One warp: dk and dv of a key row, for one head of keys and values, over the cloud's queries lo .. hi - 1; as
+// sums in f32 to `partial` (dk, then dv), if given.
 template <typename T>
 __device__ __noinline__ void attention_dkv_row(const gdl_attention &a, int hk, int64_t q0, int64_t nq, int64_t k0,
-                                               int64_t nk, int64_t row, float *sk, float *sv, const float *lse,
-                                               const float *delta, const T *dout, T *dk, T *dv) {
+                                               int64_t nk, int64_t row, int64_t lo, int64_t hi, float *sk, float *sv,
+                                               const float *lse, const float *delta, const T *dout, float *partial,
+                                               T *dk, T *dv) {
     const int lane = threadIdx.x & 31;
     const int64_t kj = k0 + row;
     const int group = a.heads / a.kv_heads;
@@ -200,7 +202,9 @@ __device__ __noinline__ void attention_dkv_row(const gdl_attention &a, int hk, i
     stage_row(sk, (const T *)a.k + kj * a.k_row + (int64_t)hk * a.k_head, a.dim);
     stage_row(sv, (const T *)a.v + kj * a.v_row + (int64_t)hk * a.v_head, a.dim);
     __syncwarp();
-    const QueryRange r = visible_queries(a, row, nq, nk);
+    QueryRange r = visible_queries(a, row, nq, nk);
+    if (r.lo < lo) r.lo = lo;
+    if (r.hi > hi) r.hi = hi;
     float ak[4] = {0.0f, 0.0f, 0.0f, 0.0f}, av[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int h = hk * group; h < (hk + 1) * group; ++h) {
         for (int64_t i0 = r.lo; i0 < r.hi; i0 += 32) {
@@ -238,8 +242,14 @@ __device__ __noinline__ void attention_dkv_row(const gdl_attention &a, int hk, i
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (lane + 32 * e < a.dim) {
-            store1(dk + ro + lane + 32 * e, ak[e] * a.scale);
-            store1(dv + ro + lane + 32 * e, av[e]);
+            const int d = lane + 32 * e;
+            if (partial) {
+                partial[d] = ak[e] * a.scale;
+                partial[a.dim + d] = av[e];
+            } else {
+                store1(dk + ro + d, ak[e] * a.scale);
+                store1(dv + ro + d, av[e]);
+            }
         }
 }
 

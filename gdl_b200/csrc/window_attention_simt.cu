@@ -4,9 +4,9 @@
 // f32 products have no tensor-core form of their precision, so these kernels are bound by FFMA: a CTA of 128
 // threads holds 64 rows against tiles of 32 columns, each thread a 4 x 4 block of the products (two 16-byte
 // shared-memory reads to 16 FFMA) and 4 x (dim / 8) of the outputs. Tiles lie transposed ([dim][row]) where
-// they are summed over dim, as they are where they are summed over rows. A column (a key; in the dK, dV kernel a
-// query) with a value that is not finite is left out of the tiles: the rows that see one are computed again,
-// row by row, from what they see. 6 ragged clouds up to 1023 rows, 4 heads of 24 over 2, window 129, 16 buckets,
+// they are summed over dim, as they are where they are summed over rows. What is not finite does not go into a
+// tile (0 times it would reach other rows): a row of the CTA that has such a value, or that sees a column (a key; in
+// the dK, dV kernel a query) with one, is computed again, by itself, from what it sees. 6 ragged clouds up to 1023 rows, 4 heads of 24 over 2, window 129, 16 buckets,
 // f32: 49 us forward, 61 us dQ, 102 us dK and dV, far from what the FFMA take: 232 CTAs of 4 warps.
 #include "attention_sinks.cuh"
 
@@ -43,16 +43,17 @@ struct Load {
             if (across) across[d * ld + lane] = x;
             if (along) along[lane * (D + 4) + d] = x;
         }
-        if (bad && odd) atomicOr(bad, 1u << lane);
+        if (odd) atomicOr(bad, 1u << lane);
     }
 };
+// The CTA's own rows; bad[2] takes those that are not finite.
 template <typename T, int D>
-__device__ __forceinline__ void load_rows(const T *p, int64_t row_stride, int n, int dim, float *across) {
+__device__ __forceinline__ void load_rows(const T *p, int64_t row_stride, int n, int dim, float *across, uint32_t *bad) {
 #pragma unroll 1
     for (int half = 0; half < kRows / 32; ++half) {
         Load<T, D> l;
         l.read(p + half * 32 * row_stride, row_stride, n - half * 32, dim);
-        l.write(across + half * 32, kRowLd, nullptr, nullptr);
+        l.write(across + half * 32, kRowLd, nullptr, bad + half);
     }
 }
 // Positions of the n columns of a tile: a value to a thread.
@@ -158,10 +159,11 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const __grid_consta
     const int64_t k0 = ragged_bound(a.ptr_k, a.num_clouds, a.n_key, t.cloud + 1);
     const int64_t k1 = ragged_bound(a.ptr_k, a.num_clouds, a.n_key, t.cloud + 2), nk = k1 > k0 ? k1 - k0 : 0;
     const int64_t off = nk - t.n;
-    load_rows<T, D>((const T *)a.q + row0 * a.q_row + (int64_t)h * a.q_head, a.q_row, rows, a.dim, Q);
+    if (tid < 2) again[tid] = 0;
+    __syncthreads();
+    load_rows<T, D>((const T *)a.q + row0 * a.q_row + (int64_t)h * a.q_head, a.q_row, rows, a.dim, Q, again);
     if (a.bias)
         for (int i = tid; i < a.buckets; i += kThreads) table[i] = bias_at(a, (int64_t)h * a.buckets + i) * kLog2e;
-    if (tid < 2) again[tid] = 0;
     int vis_lo[4], vis_hi[4];  // places within a cloud fit 32 bits
     float m[4], l[4], o[4][D / 8], px[4], py[4], pz[4];
     bool seen_bad[4];
@@ -301,8 +303,10 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t k0 = ragged_bound(a.ptr_k, a.num_clouds, a.n_key, t.cloud + 1);
     const int64_t k1 = ragged_bound(a.ptr_k, a.num_clouds, a.n_key, t.cloud + 2), nk = k1 > k0 ? k1 - k0 : 0;
     const int64_t off = nk - t.n, ro = (int64_t)a.heads * a.dim;
-    load_rows<T, D>((const T *)a.q + row0 * a.q_row + (int64_t)h * a.q_head, a.q_row, rows, a.dim, Q);
-    load_rows<T, D>(dout + row0 * ro + (int64_t)h * a.dim, ro, rows, a.dim, G);
+    if (tid < 2) again[tid] = 0;
+    __syncthreads();
+    load_rows<T, D>((const T *)a.q + row0 * a.q_row + (int64_t)h * a.q_head, a.q_row, rows, a.dim, Q, again);
+    load_rows<T, D>(dout + row0 * ro + (int64_t)h * a.dim, ro, rows, a.dim, G, again);
     for (int r = warp; r < rows; r += kThreads / 32) {
         float s = 0.0f;
         for (int d = lane; d < a.dim; d += 32) {
@@ -320,7 +324,6 @@ __global__ void __launch_bounds__(kThreads)
         if (part)
             for (int i = 0; i < a.buckets; ++i) hist[i * kThreads + tid] = 0.0f;
     }
-    if (tid < 2) again[tid] = 0;
     __syncthreads();
     int vis_lo[4], vis_hi[4];
     float ls[4], de[4], o[4][D / 8], px[4], py[4], pz[4];
@@ -378,11 +381,9 @@ __global__ void __launch_bounds__(kThreads)
             for (int j = 0; j < 4; ++j) {
                 const int c = tx * 4 + j;
                 const int key = (int)s.j + c;
-                bool see = c < n && key < vis_hi[i] && (key >= vis_lo[i] || key < a.num_sinks);
-                if (see && (bad >> c & 1)) {
-                    seen_bad[i] = true;
-                    see = false;
-                }
+                const bool see = c < n && key < vis_hi[i] && (key >= vis_lo[i] || key < a.num_sinks);
+                const bool odd = see && (bad >> c & 1);
+                seen_bad[i] |= odd;
                 float v = x[i][j] * scale2;
                 int b = 0;
                 if (a.bias && see) {
@@ -390,6 +391,9 @@ __global__ void __launch_bounds__(kThreads)
                     v += table[b];
                 }
                 x[i][j] = see && ls[i] != neg_inf() ? ex2(v - ls[i]) * (g[i][j] - de[i]) : 0.0f;
+                // For the bucket sums alone (dQ of the row is computed again): a key that is not finite leaves lse and delta
+                // finite only with weight 0.
+                if (odd && ls[i] != neg_inf()) x[i][j] = (ls[i] - ls[i]) + (de[i] - de[i]);
                 if (part) hist[b * kThreads + tid] += x[i][j];
             }
 #pragma unroll
@@ -455,9 +459,10 @@ __global__ void __launch_bounds__(kThreads)
         for (int i = tid; i < u.first_out * 2 * a.dim; i += kThreads) u.partial[i] = 0.0f;
         return;
     }
-    load_rows<T, D>((const T *)a.k + kr0 * a.k_row + (int64_t)hk * a.k_head, a.k_row, rows, a.dim, K);
-    load_rows<T, D>((const T *)a.v + kr0 * a.v_row + (int64_t)hk * a.v_head, a.v_row, rows, a.dim, V);
     if (tid < 2) again[tid] = 0;
+    __syncthreads();
+    load_rows<T, D>((const T *)a.k + kr0 * a.k_row + (int64_t)hk * a.k_head, a.k_row, rows, a.dim, K, again);
+    load_rows<T, D>((const T *)a.v + kr0 * a.v_row + (int64_t)hk * a.v_head, a.v_row, rows, a.dim, V, again);
     int vis_lo[4], vis_hi[4];
     float ok[4][D / 8], ov[4][D / 8], px[4], py[4], pz[4];
     bool seen_bad[4];
@@ -555,9 +560,8 @@ __global__ void __launch_bounds__(kThreads)
             for (int j = 0; j < 4; ++j) {
                 const int d = tx * 4 + 32 * g + j;
                 if (d >= a.dim) continue;
-                float x = ok[i][4 * g + j] * a.scale, y = ov[i][4 * g + j];
-                if (r < u.first_out) {  // a sink that sees what is not finite: so is its sum
-                    if (seen_bad[i]) x = y = __int_as_float(0x7fc00000);
+                const float x = ok[i][4 * g + j] * a.scale, y = ov[i][4 * g + j];
+                if (r < u.first_out) {
                     u.partial[(2 * r) * a.dim + d] = x;
                     u.partial[(2 * r + 1) * a.dim + d] = y;
                 } else {
@@ -565,13 +569,14 @@ __global__ void __launch_bounds__(kThreads)
                     store1(dv + at + d, y);
                 }
             }
-        if (seen_bad[i] && r >= u.first_out) atomicOr(again + (r >> 5), 1u << (r & 31));
+        if (seen_bad[i]) atomicOr(again + (r >> 5), 1u << (r & 31));
     }
     __syncthreads();
     for (int r = warp; r < rows; r += kThreads / 32)
         if (again[r >> 5] >> (r & 31) & 1)
-            attention_dkv_row<T>(a, hk, u.q0, u.nq, u.k0, u.nk, u.j0 + r, P + warp * 2 * kAttnMaxDim,
-                                 P + (warp * 2 + 1) * kAttnMaxDim, lse, delta, dout, dk, dv);
+            attention_dkv_row<T>(a, hk, u.q0, u.nq, u.k0, u.nk, u.j0 + r, u.lo, u.hi, P + warp * 2 * kAttnMaxDim,
+                                 P + (warp * 2 + 1) * kAttnMaxDim, lse, delta, dout,
+                                 r < u.first_out ? u.partial + (int64_t)r * 2 * a.dim : nullptr, dk, dv);
 }
 
 template <typename F>

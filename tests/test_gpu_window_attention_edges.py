@@ -4,7 +4,7 @@ hold what is not finite, rows that a bias masks throughout, extreme arguments.""
 import pytest
 import torch
 
-from .attention_ref import check, reference
+from .attention_ref import buckets, check, reference, visible
 from .test_gpu_window_attention import DT, call, make, verify
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
@@ -39,3 +39,111 @@ def test_bucket_sums_beside_keys_of_minus_infinity():
             check(got[n], want[n], n)
         first = got if first is None else first
         assert torch.equal(got["dbias"], first["dbias"])
+
+
+# ------------------------------------------------------------------ plain: row by row, in 64 bits
+def plain(c, window, sinks, buckets_of=None, logits32=False):
+    """{name: value} from the definition, each row from the keys that it sees alone; `logits32`: logits are held
+    in 32 bits. `sees` [Nq, Nk] is returned too."""
+    f = lambda t: t.detach().cpu().double()  # noqa: E731
+    q, k, v, do = (f(c[n]) for n in ("q", "k", "v", "dout"))
+    H, G, D = q.shape[1], q.shape[1] // k.shape[1], q.shape[2]
+    r = {"out": torch.zeros_like(q), "dq": torch.zeros_like(q), "dk": torch.zeros_like(k), "dv": torch.zeros_like(v)}
+    if "bias" in c:
+        r["dbias"] = torch.zeros(c["bias"].shape, dtype=torch.float64)
+    sees = torch.zeros(len(q), len(k), dtype=torch.bool)
+    pq, pk = c["ptr_q"].tolist(), c["ptr_k"].tolist()
+    for q0, q1, k0, k1 in zip(pq[:-1], pq[1:], pk[:-1], pk[1:]):
+        ok = visible(q1 - q0, k1 - k0, *window, sinks)
+        sees[q0:q1, k0:k1] = ok
+        for i in range(q1 - q0):
+            j = k0 + torch.nonzero(ok[i]).flatten()
+            for h in range(H):
+                s = (k[j, h // G] @ q[q0 + i, h]) / D ** 0.5
+                if "bias" in c:
+                    b = buckets_of[q0 + i, j]
+                    s = s + f(c["bias"])[h, b]
+                s = s.float().double() if logits32 else s
+                top = s.max() if len(j) else torch.tensor(0.0)
+                p = torch.exp(s - (0.0 if top == -float("inf") else top))
+                p = p / p.sum() if p.sum() != 0 else p
+                o = (p[:, None] * v[j, h // G]).sum(0)
+                ds = p * (v[j, h // G] @ do[q0 + i, h] - (do[q0 + i, h] * o).sum())
+                r["out"][q0 + i, h] = o
+                r["dq"][q0 + i, h] = (ds[:, None] * k[j, h // G]).sum(0) / D ** 0.5
+                r["dk"][j, h // G] += ds[:, None] * q[q0 + i, h] / D ** 0.5
+                r["dv"][j, h // G] += p[:, None] * do[q0 + i, h]
+                if "bias" in c:
+                    r["dbias"][h].index_add_(0, b, ds)
+    return r, sees
+
+
+def pair_buckets(c, radius, steps):
+    return buckets(c["pos_q"].cpu().numpy(), c["pos_k"].cpu().numpy(), radius, c["bias"].shape[1], steps)
+
+
+def bounds(c, n, extra=0.0):
+    """Worst-case errors: of a weight (e: logits of D products, bfloat16 roundings of P, dS and a result; `extra`
+    for the logits' own size), on the largest values that meet in each result; a key is seen by at most n rows."""
+    big = {m: float(torch.nan_to_num(c[m].float(), 0.0, 0.0, 0.0).abs().max()) for m in ("q", "k", "v", "dout")}
+    D, bf16 = c["q"].shape[2], c["q"].dtype == torch.bfloat16
+    e = 8 * 2.0 ** -8 if bf16 else 8 * (D + 8) * 2.0 ** -24 * max(1.0, big["q"] * big["k"] * D ** 0.5) + 2.0 ** -18
+    e += extra
+    ds = 2 * D * big["dout"] * big["v"]
+    return {"out": e * big["v"], "dq": e * ds * big["k"] / D ** 0.5, "dk": e * ds * big["q"] / D ** 0.5 * n,
+            "dv": e * big["dout"] * n, "dbias": e * ds * len(c["q"])}
+
+
+PATHS = {  # type, head size, queries: tensor cores, f32 tiles (two sizes), bf16 in those, few rows (all forwards; three backwards)
+    "mma": (torch.bfloat16, 64, None), "mma wide": (torch.bfloat16, 96, None), "tiles": (torch.float32, 24, None),
+    "tiles wide": (torch.float32, 72, None), "tiles bf16": (torch.bfloat16, 20, None), "few": (torch.bfloat16, 64, [9, 6]),
+    "few f32": (torch.float32, 32, [9, 6])}
+
+
+@pytest.mark.parametrize("path", list(PATHS))
+@pytest.mark.parametrize("name", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("whole", [True, False])
+def test_what_is_not_finite_reaches_what_sees_it(path, name, bad, whole):
+    """Where the definition gives a finite value so do the kernels, and where it does not, neither do they. (A row of
+    a gradient that sums over a value that is not finite may come out NaN as a whole on the tensor cores.)"""
+    dt, dim, lens_q = PATHS[path]
+    window, sinks = (20, 12), 2
+    for at in (0, 70, 99 + 3):  # a sink, a row in the middle, one of the second cloud
+        c = make(42, [99, 61], 2, 1, dim, dt, lens_q=lens_q, buckets=8)
+        rows = c[name].shape[0]
+        row = min(at, rows - 1) if lens_q is None or name in ("k", "v") else at % rows
+        c[name][row, 0, slice(None) if whole else slice(0, 1)] = bad
+        got = call(c, window, sinks)
+        want, sees = plain(c, window, sinks, pair_buckets(c, 0.4, 4))
+        tol = bounds(c, len(c["q"]))
+        loose = {n: torch.zeros(len(want[n]), dtype=torch.bool) for n in want if n != "dbias"}
+        if "tiles" not in path and path != "few f32":
+            if name == "k":
+                loose["dq"] = sees[:, row]
+            if name in ("q", "dout"):
+                loose["dk"] = loose["dv"] = sees[row]
+        for n in want:
+            g = got[n].detach().cpu().double()
+            fine = torch.isfinite(want[n])
+            assert not bool(torch.isfinite(g[~fine]).any()), (n, at, "finite where the definition is not")
+            here = fine if n == "dbias" else fine & ~loose[n][:, None, None]
+            assert bool(torch.isfinite(g[here]).all()), (n, at, "not finite where the definition is")
+            assert bool(((g - want[n])[here].abs() <= tol[n]).all()), (n, at)
+
+
+@pytest.mark.parametrize("path", ["tiles", "tiles wide", "tiles bf16", "few f32"])
+def test_keys_of_minus_infinity_take_no_part(path):
+    """As above where the tiles run without tensor cores: such a key's own dK and dV are 0."""
+    dt, dim, lens_q = PATHS[path]
+    c = make(48, [99, 61], 2, 1, dim, dt, lens_q=lens_q, buckets=8)
+    c["q"][..., 0] = 1.0
+    at = torch.tensor([1, 40, 95, 98, 99 + 55])
+    c["k"][at.cuda(), :, 0] = -float("inf")
+    got = call(c, (20, 12), 2)
+    want, _ = plain(c, (20, 12), 2, pair_buckets(c, 0.4, 4))
+    tol = bounds(c, len(c["q"]))
+    for n in ("out", "dk", "dv", "dbias"):
+        assert bool(torch.isfinite(got[n]).all()) and bool(torch.isfinite(want[n]).all()), n
+        assert float((got[n].detach().cpu().double() - want[n]).abs().max()) <= tol[n], n
+    assert float(got["dk"][at].abs().max()) == 0 and float(got["dv"][at].abs().max()) == 0
