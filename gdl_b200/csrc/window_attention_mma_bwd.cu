@@ -284,7 +284,8 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
             const float de = half_sum[0][r] + half_sum[1][r];
             const float ls = lse[(int64_t)h * a.n_query + qi];
             if (pass == 0 && half == 0 && live) delta[(int64_t)h * a.n_query + qi] = ls == neg_inf() ? 0.0f : de;
-            const float ls2 = ls * kLog2e;
+            // P = exp2(logit + shift); where every visible logit is -inf, so is the shift: P = 0, not exp2(-inf + inf)
+            const float shift = ls == neg_inf() ? ls : ls * -kLog2e;
             bool sees_bad = false;
             for (KeyTile t_now(kt); t_now.i < kt.count && ok; t_now.next(kt), parity ^= 1, ring_k.next(), ring_v.next()) {
                 const float *kp = kpos + ring_v.at * 3 * kMmaKeys;
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                     mask = t_now.mask(kCols * half, vis_lo, vis_hi, a.num_sinks);
                     cs = chunk_sets(mask);
                 }
-                const uint64_t up = pack2(-ls2, -ls2), dd = pack2(-de, -de);
+                const uint64_t up = pack2(shift, shift), dd = pack2(-de, -de);
 #pragma unroll
                 for (int k = 0; k < kCols / kChunk; ++k) {
                     uint32_t pk[kChunk / 2];
@@ -527,7 +528,8 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                     for (int e = 0; e < 2; ++e) {
                         const int64_t qc = lo + (int64_t)read_c * kMmaKeys + lane + 32 * e, qi = qc < nq ? qc : nq - 1;
                         const int64_t at = (int64_t)read_h * a.n_query + q0 + qi;
-                        val[e][3] = lse[at] * -kLog2e;
+                        const float ls = lse[at];
+                        val[e][3] = ls == neg_inf() ? ls : ls * -kLog2e;  // (as in dQ)
                         val[e][4] = -delta[at];
                         if (BIAS)
 #pragma unroll

@@ -147,3 +147,22 @@ def test_keys_of_minus_infinity_take_no_part(path):
         assert bool(torch.isfinite(got[n]).all()) and bool(torch.isfinite(want[n]).all()), n
         assert float((got[n].detach().cpu().double() - want[n]).abs().max()) <= tol[n], n
     assert float(got["dk"][at].abs().max()) == 0 and float(got["dv"][at].abs().max()) == 0
+
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [20, 64, 96])
+@pytest.mark.parametrize("window,sinks,lens_q", [((30, 0), 3, None), ((-1, 0), 0, None), ((12, 9), 70, None), ((25, 0), 2, [5, 3])])
+def test_buckets_of_minus_infinity(dt, dim, window, sinks, lens_q):
+    """A table that cuts off distances by -inf: a row may see such keys alone (the first of a causal cloud sees
+    itself). Its output is 0, and it takes no part in a gradient."""
+    c = make(43, [150, 40], 2, 1, dim, DT[dt], lens_q=lens_q, buckets=8)
+    c["bias"][0, 0] = c["bias"][1, 0] = -float("inf")   # not itself
+    c["bias"][0, 4:] = c["bias"][1, 1:] = -float("inf")  # not far ones; the second head sees nothing at all
+    got = call(c, window, sinks)
+    want, _ = plain(c, window, sinks, pair_buckets(c, 0.4, 4))
+    tol = bounds(c, len(c["q"]))
+    for n in want:
+        assert bool(torch.isfinite(got[n]).all()), n
+        assert float((got[n].detach().cpu().double() - want[n]).abs().max()) <= tol[n], n
+    assert float(got["out"][:, 1].abs().max()) == 0 and float(got["dq"][:, 1].abs().max()) == 0
