@@ -649,6 +649,7 @@ def window_attention_cuda(q, k, v, bias, ptr_q, ptr_k, window, num_sinks, scale,
         pos_q = pos_k = None
     ptr_q, ptr_k = _bounds(ptr_q, dev), _bounds(ptr_k, dev)
     held = (_head_rows(q), _head_rows(k), _head_rows(v), bias, ptr_q, ptr_k, pos_q, pos_k)
+    left, right = min(left, 2**62), min(right, 2**62)  # (any number of rows is fewer)
     meta = (left, right, min(int(num_sinks), 2**31 - 1), float(scale), inv_r2, steps_log2)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(H, q.shape[0], dtype=torch.float32, device=dev) if with_lse else None

@@ -48,6 +48,16 @@ int check(const gdl_attention *a) {
     return GDL_OK;
 }
 
+// The same windows in numbers that leave room for sums of places: a side that reaches over all rows is open, and
+// where every key is a sink (or the left side is open) there is nothing for sinks to do.
+gdl_attention normal(const gdl_attention &given) {
+    gdl_attention a = given;
+    if (a.left >= a.n_key || a.num_sinks >= a.n_key) a.left = -1;
+    if (a.right >= a.n_key + a.n_query) a.right = -1;
+    if (a.left < 0) a.num_sinks = 0;
+    return a;
+}
+
 // Which kernels take a call: few rows stream the window (window_attention_stream.cu), bf16 in layouts that TMA
 // can read goes to the tensor cores (window_attention_mma*.cu), everything else (f32, head sizes that are no
 // multiple of 8, unaligned views) to the FFMA tiles (window_attention_simt.cu).
@@ -79,46 +89,50 @@ size_t part_bytes(const gdl_attention &a) {
 
 using namespace gdl;
 
-extern "C" int gdl_window_attention(const gdl_attention *a, void *out, float *lse, void *out_rest, void *stream) {
-    const int rc = check(a);
+extern "C" int gdl_window_attention(const gdl_attention *given, void *out, float *lse, void *out_rest, void *stream) {
+    const int rc = check(given);
     if (rc != GDL_OK) return rc;
-    if (a->n_query == 0) return GDL_OK;
+    const gdl_attention a = normal(*given);
+    if (a.n_query == 0) return GDL_OK;
     GDL_RETURN_IF(!out, GDL_ERR_INVALID);
     cudaStream_t st = (cudaStream_t)stream;
-    GDL_RETURN_IF(out_rest && a->dtype != GDL_DTYPE_BF16, GDL_ERR_INVALID);
-    const bool few = takes_stream(*a);
-    if (!few && takes_mma(*a) && (((uintptr_t)out | (uintptr_t)out_rest) & 15) == 0)
-        return attention_forward_mma(*a, (uint16_t *)out, lse, (uint16_t *)out_rest, st);
-    if (out_rest) GDL_CUDA_TRY(cudaMemsetAsync(out_rest, 0, (size_t)a->n_query * a->heads * a->dim * 2, st));
-    if (few) return attention_forward_stream(*a, out, lse, st);
-    return attention_forward_simt(*a, out, lse, st);
+    GDL_RETURN_IF(out_rest && a.dtype != GDL_DTYPE_BF16, GDL_ERR_INVALID);
+    const bool few = takes_stream(a);
+    if (!few && takes_mma(a) && (((uintptr_t)out | (uintptr_t)out_rest) & 15) == 0)
+        return attention_forward_mma(a, (uint16_t *)out, lse, (uint16_t *)out_rest, st);
+    if (out_rest) GDL_CUDA_TRY(cudaMemsetAsync(out_rest, 0, (size_t)a.n_query * a.heads * a.dim * 2, st));
+    if (few) return attention_forward_stream(a, out, lse, st);
+    return attention_forward_simt(a, out, lse, st);
 }
 
-extern "C" size_t gdl_window_attention_backward_workspace_size(const gdl_attention *a) {
-    if (check(a) != GDL_OK) return 256;
-    const size_t sinks = attention_backward_simt_workspace(*a), mma = attention_backward_mma_workspace(*a);
-    return delta_bytes(*a) + part_bytes(*a) + (sinks > mma ? sinks : mma) + 256;
+extern "C" size_t gdl_window_attention_backward_workspace_size(const gdl_attention *given) {
+    if (check(given) != GDL_OK) return 256;
+    const gdl_attention a = normal(*given);
+    const size_t sinks = attention_backward_simt_workspace(a), mma = attention_backward_mma_workspace(a);
+    return delta_bytes(a) + part_bytes(a) + (sinks > mma ? sinks : mma) + 256;
 }
 
-extern "C" int gdl_window_attention_backward(const gdl_attention *a, const void *out, const float *lse,
-                                             const void *out_rest, const void *grad_out, void *dq, void *dk, void *dv, void *dbias,
-                                             void *workspace, size_t workspace_bytes, void *stream) {
-    const int rc = check(a);
+extern "C" int gdl_window_attention_backward(const gdl_attention *given, const void *out, const float *lse,
+                                             const void *out_rest, const void *grad_out, void *dq, void *dk, void *dv,
+                                             void *dbias, void *workspace, size_t workspace_bytes, void *stream) {
+    const int rc = check(given);
     if (rc != GDL_OK) return rc;
-    GDL_RETURN_IF(a->n_query > 0 && (!out || !lse || !grad_out || !dq), GDL_ERR_INVALID);
-    GDL_RETURN_IF(a->n_key > 0 && (!dk || !dv), GDL_ERR_INVALID);
-    GDL_RETURN_IF(dbias && !a->bias, GDL_ERR_INVALID);
-    GDL_RETURN_IF(!workspace || workspace_bytes < gdl_window_attention_backward_workspace_size(a), GDL_ERR_WORKSPACE);
+    const gdl_attention a = normal(*given);
+    GDL_RETURN_IF(a.n_query > 0 && (!out || !lse || !grad_out || !dq), GDL_ERR_INVALID);
+    GDL_RETURN_IF(a.n_key > 0 && (!dk || !dv), GDL_ERR_INVALID);
+    GDL_RETURN_IF(dbias && !a.bias, GDL_ERR_INVALID);
+    GDL_RETURN_IF(!workspace || workspace_bytes < gdl_window_attention_backward_workspace_size(given), GDL_ERR_WORKSPACE);
     cudaStream_t st = (cudaStream_t)stream;
     char *ws = (char *)workspace;
-    float *delta = (float *)ws, *part = dbias ? (float *)(ws + delta_bytes(*a)) : nullptr;
-    float *sinks = (float *)(ws + delta_bytes(*a) + part_bytes(*a));
+    float *delta = (float *)ws, *part = dbias ? (float *)(ws + delta_bytes(a)) : nullptr;
+    float *sinks = (float *)(ws + delta_bytes(a) + part_bytes(a));
     const uintptr_t all = (uintptr_t)out | (uintptr_t)out_rest | (uintptr_t)grad_out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
-    const bool mma = takes_mma(*a) && (all & 15) == 0;
-    const int done = mma ? attention_backward_mma(*a, (const uint16_t *)out, lse, (const uint16_t *)out_rest, (const uint16_t *)grad_out, (uint16_t *)dq,
-                                                  (uint16_t *)dk, (uint16_t *)dv, delta, part, sinks, st)
-                         : attention_backward_simt(*a, out, lse, out_rest, grad_out, dq, dk, dv, delta, part, sinks, st);
+    const bool mma = takes_mma(a) && (all & 15) == 0;
+    const int done = mma ? attention_backward_mma(a, (const uint16_t *)out, lse, (const uint16_t *)out_rest,
+                                                  (const uint16_t *)grad_out, (uint16_t *)dq, (uint16_t *)dk,
+                                                  (uint16_t *)dv, delta, part, sinks, st)
+                         : attention_backward_simt(a, out, lse, out_rest, grad_out, dq, dk, dv, delta, part, sinks, st);
     if (done != GDL_OK || !dbias) return done;
-    const int64_t parts = ragged_slots(a->n_query, a->num_clouds, mma ? kMmaRows : attention_simt_rows());
-    return reduce_bias(*a, part, a->n_query > 0 ? parts : 0, dbias, st);
+    const int64_t parts = ragged_slots(a.n_query, a.num_clouds, mma ? kMmaRows : attention_simt_rows());
+    return reduce_bias(a, part, a.n_query > 0 ? parts : 0, dbias, st);
 }

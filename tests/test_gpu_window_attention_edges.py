@@ -1,6 +1,8 @@
 """Windowed attention on the GPU where single rows go wrong: maxima that keep growing, rows and columns that
 hold what is not finite, rows that a bias masks throughout, extreme arguments."""
 
+import sys
+
 import pytest
 import torch
 
@@ -166,3 +168,15 @@ def test_buckets_of_minus_infinity(dt, dim, window, sinks, lens_q):
         assert bool(torch.isfinite(got[n]).all()), n
         assert float((got[n].detach().cpu().double() - want[n]).abs().max()) <= tol[n], n
     assert float(got["out"][:, 1].abs().max()) == 0 and float(got["dq"][:, 1].abs().max()) == 0
+
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_largest_windows_and_sinks_are_open_ones(dt):
+    c = make(45, [200, 33], 2, 1, 32, DT[dt])
+    for big in (sys.maxsize, 2 ** 62, 2 ** 70):
+        for window, sinks, same in (((big, big), 0, (-1, -1)), ((big, 0), 0, (-1, 0)), ((10, big), 0, (10, -1)),
+                                    ((10, 5), big, (-1, 5)), ((big, 5), big, (-1, 5))):
+            got, want = call(c, window, sinks), call(c, same, 0)
+            for n in want:
+                assert torch.equal(got[n], want[n]), (n, window, sinks)
