@@ -29,6 +29,8 @@ constexpr int kChainWarps = 32;
 // Calls of so few rows run in one launch, a thread to a channel of a cloud: 3 launches take longer than a few
 // rows in turn (64 clouds of one row, 256 channels: 2.4 us).
 constexpr int64_t kSerialRows = 256;
+constexpr int kSerialClouds = 65533;  // (with the rows of no cloud, the y of a grid)
+bool takes_serial(int64_t n_rows, int32_t clouds) { return n_rows <= kSerialRows && clouds <= kSerialClouds; }
 
 __device__ __forceinline__ float rcp(float x) {
     float r;
@@ -641,7 +643,7 @@ extern "C" size_t gdl_gated_scan_states_size(int64_t n_rows, int32_t num_clouds,
 }
 
 extern "C" size_t gdl_gated_scan_workspace_size(int64_t n_rows, int32_t num_clouds, int32_t channels) {
-    if (n_rows < 0 || num_clouds < 0 || channels < 0 || n_rows <= kSerialRows) return 256;
+    if (n_rows < 0 || num_clouds < 0 || channels < 0 || takes_serial(n_rows, num_clouds)) return 256;
     return scan_space(n_rows, num_clouds, channels, false).total;
 }
 
@@ -659,7 +661,7 @@ extern "C" int gdl_gated_scan(const void *x, const void *gate, int32_t dtype, co
     if (rc != GDL_OK || channels == 0) return rc;
     GDL_RETURN_IF(n_rows > 0 && (!x || !gate || !h), GDL_ERR_INVALID);
     const int C = channels, B = num_clouds;
-    if (n_rows <= kSerialRows && B <= 65533) {
+    if (takes_serial(n_rows, B)) {
         const dim3 grid((C + kScanThreads - 1) / kScanThreads, B + 2);
         if (dtype == GDL_DTYPE_F32)
             scan_serial_kernel<float><<<grid, kScanThreads, 0, st>>>((const float *)x, (const float *)gate, decay, ptr, B,

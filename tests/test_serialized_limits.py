@@ -45,3 +45,10 @@ def test_bounds_on_another_gpu_are_copied(monkeypatch):
     there = Bounds()
     assert csrc._bounds(there, torch.device("cuda", 0)) == ("copied", torch.device("cuda", 0))
     assert csrc._bounds(there, torch.device("cuda", 1)) is there
+
+
+def test_few_rows_of_many_clouds_are_given_a_workspace(lib):  # noqa: F811
+    """The size asked for is that of the kernels that run: one launch takes few rows of up to 65533 clouds."""
+    assert lib.gdl_gated_scan_workspace_size(256, 65533, 8) == 256
+    assert lib.gdl_gated_scan_workspace_size(256, 65534, 8) > 65534 * 8 * 4
+    assert lib.gdl_gated_scan_workspace_size(0, 70000, 8) > 70000 * 8 * 4
