@@ -92,7 +92,7 @@ class SerializedAttention(nn.Module):
         q, k, v = rows.split([self.heads, self.kv_heads, self.kv_heads], 1)  # views: no copy
         y = window_attention(q, k, v, ptr, window=self.window, num_sinks=self.sinks, bias=self.bias, pos_q=pos,
                              radius=self.radius, steps=self.steps)
-        return self.outer(y.reshape(x.shape[0], -1))
+        return self.outer(y.flatten(1))
 
 
 class SerializedBlock(nn.Module):
