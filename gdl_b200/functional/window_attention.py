@@ -22,9 +22,10 @@ class WindowAttention(torch.autograd.Function):
     """out of gdl_window_attention; differentiable w.r.t. q, k, v and the bias table."""
 
     @staticmethod
-    def forward(ctx, q: Tensor, k: Tensor, v: Tensor, bias: Optional[Tensor], meta):
-        need = any(ctx.needs_input_grad[:4])
-        out, lse, rest, args = csrc.window_attention_cuda(q, k, v, bias, *meta, with_lse=need)
+    def forward(ctx, q: Tensor, k: Tensor, v: Tensor, bias: Optional[Tensor], pos_q: Optional[Tensor],
+                pos_k: Optional[Tensor], meta, train: bool):
+        need = train and any(ctx.needs_input_grad[:4])
+        out, lse, rest, args = csrc.window_attention_cuda(q, k, v, bias, *meta[:5], pos_q, pos_k, *meta[5:], with_lse=need)
         if need:
             q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k = args[0]
             ctx.save_for_backward(out, lse, rest, q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k)
@@ -37,7 +38,7 @@ class WindowAttention(torch.autograd.Function):
         out, lse, rest, *held = ctx.saved_tensors
         dq, dk, dv, db = csrc.window_attention_backward_cuda(held, ctx.meta, out, lse, rest, grad_out,
                                                              want_bias=ctx.needs_input_grad[3])
-        return dq, dk, dv, db, None
+        return dq, dk, dv, db, None, None, None, None
 
 
 def window_attention(q: Tensor, k: Tensor, v: Tensor, ptr_q: Tensor, *, ptr_k: Optional[Tensor] = None,
@@ -63,8 +64,5 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, ptr_q: Tensor, *, ptr_k: O
     if (pos_q is not None and pos_q.requires_grad) or (pos_k is not None and pos_k.requires_grad):
         raise csrc.nat.GdlError("window_attention: positions are constants of the bias; detach them")
     meta = (ptr_q, ptr_q if ptr_k is None else ptr_k, window, num_sinks,
-            1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None else scale, pos_q, pos_q if pos_k is None else pos_k,
-            radius, steps)
-    if torch.is_grad_enabled():
-        return WindowAttention.apply(q, k, v, bias, meta)
-    return csrc.window_attention_cuda(q, k, v, bias, *meta, with_lse=False)[0]
+            1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None else scale, radius, steps)
+    return WindowAttention.apply(q, k, v, bias, pos_q, pos_q if pos_k is None else pos_k, meta, torch.is_grad_enabled())

@@ -1,7 +1,10 @@
-"""Gated scan on the GPU: many clouds of few rows."""
+"""Gated scan on the GPU: many clouds of few rows, tangents."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
+
+from gdl_b200.functional import gated_scan
 
 from .test_gpu_gated_scan import DT, call, make
 
@@ -25,3 +28,11 @@ def test_more_clouds_than_a_grid_has_rows(dt, reverse):
         assert float((a - b).abs().max()) <= tol * 4 * float(b.abs().max()), n
     assert torch.equal(got["last"][len(lens):].cpu(), many["h0"][len(lens):])
     assert torch.equal(got["dh0"][len(lens):].cpu(), many["dlast"][len(lens):])
+
+
+def test_a_tangent_is_refused_without_gradients_too():
+    c = make(21, [40], 8, torch.float32)
+    x, gate, decay, ptr = (c[m].cuda() for m in ("x", "gate", "decay", "ptr"))
+    with torch.no_grad(), fwAD.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            gated_scan(fwAD.make_dual(x, torch.ones_like(x)), gate, decay, ptr)

@@ -5,6 +5,9 @@ import sys
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
+
+from gdl_b200.functional import window_attention
 
 from .attention_ref import buckets, check, reference, visible
 from .test_gpu_window_attention import DT, call, make, verify
@@ -180,3 +183,24 @@ def test_largest_windows_and_sinks_are_open_ones(dt):
             got, want = call(c, window, sinks), call(c, same, 0)
             for n in want:
                 assert torch.equal(got[n], want[n]), (n, window, sinks)
+
+
+
+def test_a_tangent_is_refused_without_gradients_too():
+    c = make(47, [40], 2, 2, 16, torch.float32)
+    with torch.no_grad(), fwAD.dual_level():
+        q = fwAD.make_dual(c["q"], torch.ones_like(c["q"]))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            window_attention(q, c["k"], c["v"], c["ptr_q"], window=(4, 4))
+        with pytest.raises((RuntimeError, NotImplementedError)):  # positions are constants: not of a tangent either
+            window_attention(c["q"], c["k"], c["v"], c["ptr_q"], window=(4, 4), bias=torch.zeros(2, 4).cuda(),
+                             pos_q=fwAD.make_dual(torch.rand(40, 3).cuda(), torch.ones(40, 3).cuda()))
+
+
+def test_nothing_is_kept_without_gradients():
+    c = make(49, [40], 2, 2, 16, torch.float32)
+    q = c["q"].requires_grad_(True)
+    with torch.no_grad():
+        out = window_attention(q, c["k"], c["v"], c["ptr_q"], window=(4, 4))
+    assert not out.requires_grad and out.grad_fn is None
+    assert torch.equal(out, window_attention(q, c["k"], c["v"], c["ptr_q"], window=(4, 4)))
