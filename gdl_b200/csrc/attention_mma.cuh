@@ -249,12 +249,10 @@ bool takes_stream(const gdl_attention &a);
 int attention_forward_stream(const gdl_attention &a, void *out, float *lse, cudaStream_t st);
 int attention_simt_rows();
 int attention_forward_simt(const gdl_attention &a, void *out, float *lse, cudaStream_t st);
-size_t attention_backward_simt_workspace(const gdl_attention &a);
 int attention_backward_simt(const gdl_attention &a, const void *out, const float *lse, const void *rest, const void *dout, void *dq, void *dk,
-                            void *dv, float *delta, float *part, float *sink_ws, cudaStream_t st);
-size_t attention_backward_mma_workspace(const gdl_attention &a);
+                            void *dv, float *delta, float *part, float *sink_ws, int chunk, cudaStream_t st);
 int attention_backward_mma(const gdl_attention &a, const uint16_t *out, const float *lse, const uint16_t *rest, const uint16_t *dout,
                            uint16_t *dq, uint16_t *dk, uint16_t *dv, float *delta, float *part, float *sink_ws,
-                           cudaStream_t st);
+                           int chunk, cudaStream_t st);
 
 }  // namespace gdl

@@ -9,13 +9,19 @@
 
 namespace gdl {
 
+// Partial sums lie in rows of [2][dim] floats (dK, dV), for each key head: a cloud's sinks take as many as it has, so
+// that cloud b starts at min(b * sinks, its first key) and no two overlap; chunk i of a cloud's queries takes them
+// (first query / size + i) * sinks rows further on.
 struct SinkPlan {
-    int tiles;      // key tiles with sinks in them
-    int rows;       // rows of one partial
-    int size;       // queries of a chunk
-    int64_t slots;  // chunks (slots of a ragged tiling)
+    int tiles;       // key tiles with sinks in them
+    int sinks, size; // sinks of a cloud at most; queries of a chunk
+    int64_t slots;   // chunks (slots of a ragged tiling)
+    int64_t main_rows, chunk_rows;  // of one key head
     float *main, *chunk;
 };
+__device__ __forceinline__ int64_t sink_base(const SinkPlan &sp, int64_t cloud, int64_t k0) {
+    return cloud * sp.sinks < k0 ? cloud * sp.sinks : k0;
+}
 
 // queries of a cloud that the window alone lets see keys up to j1: the end of a tile's own range
 __device__ __forceinline__ int64_t window_end(const gdl_attention &a, int64_t j1, int64_t nq, int64_t nk) {
@@ -24,22 +30,27 @@ __device__ __forceinline__ int64_t window_end(const gdl_attention &a, int64_t j1
     return e < 0 ? 0 : e > nq ? nq : e;
 }
 
+// `chunk`: queries of a chunk where sinks are few. With many it grows, so that the chunks of all queries together have
+// no more rows than there are keys (131072 rows, 4 key heads of 64, 2048 sinks: 0.27 GB in chunks of 2048).
 inline SinkPlan sink_plan(const gdl_attention &a, float *ws, int tile_rows, int chunk) {
     SinkPlan sp = {};
     if (a.left < 0 || a.num_sinks == 0 || a.n_key == 0 || a.n_query == 0) return sp;
-    const int64_t sinks = a.num_sinks < a.n_key ? a.num_sinks : a.n_key;
-    sp.tiles = (int)((sinks + tile_rows - 1) / tile_rows);
-    sp.rows = (int)(sinks < tile_rows ? sinks : tile_rows);
-    sp.size = chunk;
-    sp.slots = ragged_slots(a.n_query, a.num_clouds, chunk);
-    const int64_t size = (int64_t)sp.rows * 2 * a.dim * sp.tiles * a.kv_heads;
+    sp.sinks = (int)(a.num_sinks < a.n_key ? a.num_sinks : a.n_key);
+    sp.tiles = (sp.sinks + tile_rows - 1) / tile_rows;
+    const int64_t least = (a.n_query * sp.sinks + a.n_key - 1) / a.n_key;
+    const int64_t size = (least + chunk - 1) / chunk * chunk;
+    sp.size = (int)(size < ((int64_t)1 << 30) ? size : (int64_t)1 << 30);
+    sp.slots = ragged_slots(a.n_query, a.num_clouds, sp.size);
+    const int64_t every = (int64_t)a.num_clouds * sp.sinks;
+    sp.main_rows = every < a.n_key ? every : a.n_key;
+    sp.chunk_rows = a.n_query / sp.size * sp.sinks + sp.main_rows;
     sp.main = ws;
-    sp.chunk = ws ? ws + a.num_clouds * size : nullptr;
+    sp.chunk = ws ? ws + sp.main_rows * a.kv_heads * 2 * a.dim : nullptr;
     return sp;
 }
-inline size_t sink_bytes(const gdl_attention &a, int tile_rows, int chunk) {
-    const SinkPlan sp = sink_plan(a, nullptr, tile_rows, chunk);
-    return (size_t)(a.num_clouds + sp.slots) * sp.rows * 2 * a.dim * sp.tiles * a.kv_heads * sizeof(float);
+inline size_t sink_bytes(const gdl_attention &a, int chunk) {
+    const SinkPlan sp = sink_plan(a, nullptr, 1, chunk);
+    return (size_t)(sp.main_rows + sp.chunk_rows) * a.kv_heads * 2 * a.dim * sizeof(float);
 }
 
 // What a CTA does: CTAs 0 .. main - 1 are the key tiles (slot * kv_heads + head), then the sinks' chunks.
@@ -74,7 +85,8 @@ __device__ __forceinline__ SinkUnit sink_unit(const gdl_attention &a, const Sink
         u.lo = end > t.first ? end : t.first;
         u.hi = t.first + sp.size < u.nq ? t.first + sp.size : u.nq;
         if (u.hi <= u.lo) return u;  // the last kernel skips it by the same rule
-        u.partial = sp.chunk + unit * sp.rows * 2 * a.dim;
+        u.partial = sp.chunk + (u.hk * sp.chunk_rows + (u.q0 / sp.size + t.first / sp.size) * sp.sinks +
+                                sink_base(sp, t.cloud, u.k0) + u.j0) * 2 * a.dim;
     } else {
         const Tile t = ragged_tile(a.ptr_k, a.num_clouds, a.n_key, tile_rows, unit / a.kv_heads);
         if (t.cloud == -2) return u;
@@ -89,7 +101,7 @@ __device__ __forceinline__ SinkUnit sink_unit(const gdl_attention &a, const Sink
             u.lo = visible_queries(a, u.j0, u.nq, u.nk).lo;
             u.hi = window_end(a, u.j0 + u.rows - 1, u.nq, u.nk);
             if (sp.tiles > 0 && u.j0 < a.num_sinks) {
-                u.partial = sp.main + (((int64_t)t.cloud * sp.tiles + u.j0 / tile_rows) * a.kv_heads + u.hk) * sp.rows * 2 * a.dim;
+                u.partial = sp.main + (u.hk * sp.main_rows + sink_base(sp, t.cloud, u.k0) + u.j0) * 2 * a.dim;
                 u.first_out = (int)(a.num_sinks - u.j0 < u.rows ? a.num_sinks - u.j0 : u.rows);
             }
         }
@@ -113,12 +125,11 @@ static __global__ void __launch_bounds__(256)
     const int64_t j0 = (int64_t)s * tile_rows, j1 = j0 + tile_rows < nk ? j0 + tile_rows : nk;
     const int64_t js = j1 < a.num_sinks ? j1 : a.num_sinks;
     if (js <= j0) return;
-    const int64_t size = (int64_t)sp.rows * 2 * a.dim, end = window_end(a, j1 - 1, nq, nk);
-    const float *main = sp.main + (((int64_t)b * sp.tiles + s) * a.kv_heads + hk) * size;
-    const int64_t slot0 = q0 / sp.size + b + 1;  // of the cloud's first chunk
-    const int64_t first = end < nq ? slot0 + end / sp.size : 0, last = end < nq ? slot0 + (nq - 1) / sp.size + 1 : 0;
-    const int64_t step = (int64_t)sp.tiles * a.kv_heads * size;
-    const float *chunk = sp.chunk + ((int64_t)s * a.kv_heads + hk) * size;
+    const int64_t end = window_end(a, j1 - 1, nq, nk), at = sink_base(sp, b, k0) + j0;
+    const float *main = sp.main + (hk * sp.main_rows + at) * 2 * a.dim;
+    const int64_t first = end < nq ? end / sp.size : 0, last = end < nq ? (nq - 1) / sp.size + 1 : 0;
+    const int64_t step = (int64_t)sp.sinks * 2 * a.dim;
+    const float *chunk = sp.chunk + (hk * sp.chunk_rows + q0 / sp.size * sp.sinks + at) * 2 * a.dim;
     for (int i = blockIdx.y * 256 + threadIdx.x; i < (int)(js - j0) * 2 * a.dim; i += gridDim.y * 256) {
         float sum = main[i];
 #pragma unroll 8
@@ -130,8 +141,10 @@ static __global__ void __launch_bounds__(256)
 template <typename T>
 int join_sinks(const gdl_attention &a, const SinkPlan &sp, int tile_rows, T *dk, T *dv, cudaStream_t st) {
     if (sp.tiles == 0 || a.num_clouds == 0) return GDL_OK;
-    const int blocks = (sp.rows * 2 * a.dim + 255) / 256;
-    attn_sink_join_kernel<T><<<dim3((unsigned)(a.num_clouds * sp.tiles * a.kv_heads), blocks), 256, 0, st>>>(a, sp, tile_rows, dk, dv);
+    const int64_t ctas = (int64_t)a.num_clouds * sp.tiles * a.kv_heads;
+    GDL_RETURN_IF(ctas > ((int64_t)1 << 31) - 1, GDL_ERR_OVERFLOW);
+    const int rows = sp.sinks < tile_rows ? sp.sinks : tile_rows, blocks = (rows * 2 * a.dim + 255) / 256;
+    attn_sink_join_kernel<T><<<dim3((unsigned)ctas, blocks), 256, 0, st>>>(a, sp, tile_rows, dk, dv);
     GDL_CUDA_TRY(cudaGetLastError());
     return GDL_OK;
 }

@@ -1,6 +1,6 @@
 // window_attention.cu -- attention over packed clouds with a sliding window, sinks and a distance bias:
 // argument checks, the choice of the kernels, and the last sum of the bias gradient.
-#include "attention_mma.cuh"
+#include "attention_sinks.cuh"
 
 namespace gdl {
 namespace {
@@ -78,6 +78,10 @@ int reduce_bias(const gdl_attention &a, const float *part, int64_t parts, void *
     return GDL_OK;
 }
 
+// Queries of a chunk of the sinks': 16 tiles on the tensor cores, 4 in the FFMA tiles (8: 131 instead of 101 us for dK,
+// dV of 6 ragged clouds up to 1023 rows, 4 heads of 24 over 2). By the inputs alone, as the workspace is asked for.
+int sink_chunk(const gdl_attention &a) { return takes_mma(a) ? 1024 : 128; }
+
 // workspace: delta [heads, n_query], the bucket sums of each slot of query rows, the sinks' partial sums
 size_t delta_bytes(const gdl_attention &a) { return align256((size_t)a.heads * a.n_query * 4); }
 size_t part_bytes(const gdl_attention &a) {
@@ -108,8 +112,7 @@ extern "C" int gdl_window_attention(const gdl_attention *given, void *out, float
 extern "C" size_t gdl_window_attention_backward_workspace_size(const gdl_attention *given) {
     if (check(given) != GDL_OK) return 256;
     const gdl_attention a = normal(*given);
-    const size_t sinks = attention_backward_simt_workspace(a), mma = attention_backward_mma_workspace(a);
-    return delta_bytes(a) + part_bytes(a) + (sinks > mma ? sinks : mma) + 256;
+    return delta_bytes(a) + part_bytes(a) + sink_bytes(a, sink_chunk(a)) + 256;
 }
 
 extern "C" int gdl_window_attention_backward(const gdl_attention *given, const void *out, const float *lse,
@@ -130,8 +133,8 @@ extern "C" int gdl_window_attention_backward(const gdl_attention *given, const v
     const bool mma = takes_mma(a) && (all & 15) == 0;
     const int done = mma ? attention_backward_mma(a, (const uint16_t *)out, lse, (const uint16_t *)out_rest,
                                                   (const uint16_t *)grad_out, (uint16_t *)dq, (uint16_t *)dk,
-                                                  (uint16_t *)dv, delta, part, sinks, st)
-                         : attention_backward_simt(a, out, lse, out_rest, grad_out, dq, dk, dv, delta, part, sinks, st);
+                                                  (uint16_t *)dv, delta, part, sinks, sink_chunk(a), st)
+                         : attention_backward_simt(a, out, lse, out_rest, grad_out, dq, dk, dv, delta, part, sinks, sink_chunk(a), st);
     if (done != GDL_OK || !dbias) return done;
     const int64_t parts = ragged_slots(a.n_query, a.num_clouds, mma ? kMmaRows : attention_simt_rows());
     return reduce_bias(a, part, a.n_query > 0 ? parts : 0, dbias, st);

@@ -20,7 +20,6 @@ using namespace tc;
 constexpr int kBwdSoft = 256;               // softmax threads: 8 warps
 constexpr int kBwdThreads = kBwdSoft + 32;  // and the warp that loads and issues the products
 constexpr int kCols = 32;                   // columns of a tile that one thread handles
-constexpr int kSinkChunk = 1024;            // queries of a chunk of the sinks' (16 tiles)
 
 __device__ __forceinline__ float dot8(const uint4 &x, const uint4 &y) {
     const uint32_t p[4] = {x.x, x.y, x.z, x.w}, q[4] = {y.x, y.y, y.z, y.w};
@@ -780,14 +779,11 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
 
 }  // namespace
 
-size_t attention_backward_mma_workspace(const gdl_attention &a) {
-    return sink_bytes(a, kMmaRows, kSinkChunk);
-}
-
-// delta [heads, n_query]; part: the bucket sums of each slot of 128 query rows (nullable); sink_ws as above
+// delta [heads, n_query]; part: the bucket sums of each slot of 128 query rows (nullable); sink_ws: the partial sums of
+// chunks of `chunk` queries
 int attention_backward_mma(const gdl_attention &a, const uint16_t *out, const float *lse, const uint16_t *rest,
                            const uint16_t *dout, uint16_t *dq, uint16_t *dk, uint16_t *dv, float *delta, float *part, float *sink_ws,
-                           cudaStream_t st) {
+                           int chunk, cudaStream_t st) {
     const int nb = a.bias ? a.buckets : 0;
     const int64_t dh = a.dim, dr = (int64_t)a.heads * a.dim;
     CUtensorMap mq, mk, mv, md;
@@ -797,7 +793,7 @@ int attention_backward_mma(const gdl_attention &a, const uint16_t *out, const fl
         !head_map(&md, dout, a.dim, a.heads, a.n_query, dh, dr, kMmaRows))
         return GDL_ERR_CUDA;
     const int64_t q_ctas = ragged_slots(a.n_query, a.num_clouds, kMmaRows) * a.heads;
-    const SinkPlan sp = sink_plan(a, sink_ws, kMmaRows, kSinkChunk);
+    const SinkPlan sp = sink_plan(a, sink_ws, kMmaRows, chunk);
     const int64_t k_ctas = ragged_slots(a.n_key, a.num_clouds, kMmaRows) * a.kv_heads;
     const int64_t s_ctas = sp.tiles * sp.slots * a.kv_heads, top = ((int64_t)1 << 31) - 1;
     GDL_RETURN_IF(q_ctas > top || k_ctas + s_ctas > top, GDL_ERR_OVERFLOW);

@@ -14,7 +14,6 @@ namespace gdl {
 namespace {
 
 constexpr int kRows = 64, kCols = 32, kThreads = 128;
-constexpr int kSinkChunk = 128;  // queries of a chunk of the sinks' (4 tiles; 256: 131 instead of 101 us for dK, dV at the size above)
 constexpr int kRowLd = kRows + 4, kColLd = kCols + 4;  // (16-byte rows, odd multiple of 16 bytes)
 
 // 32 rows of a [rows][heads][dim] tensor on their way into tiles: all loads of a thread first, then the stores.
@@ -600,8 +599,8 @@ int forward(const gdl_attention &a, T *out, float *lse, cudaStream_t st) {
 
 template <typename T>
 int backward(const gdl_attention &a, const T *out, const float *lse, const T *rest, const T *dout, T *dq, T *dk, T *dv, float *delta,
-             float *part, float *sink_ws, cudaStream_t st) {
-    const SinkPlan sp = sink_plan(a, sink_ws, kRows, kSinkChunk);
+             float *part, float *sink_ws, int chunk, cudaStream_t st) {
+    const SinkPlan sp = sink_plan(a, sink_ws, kRows, chunk);
     return by_dim(a.dim, [&](auto d) -> int {
         constexpr int D = decltype(d)::value;
         const int nb = a.bias ? a.buckets : 0;
@@ -632,14 +631,13 @@ int attention_forward_simt(const gdl_attention &a, void *out, float *lse, cudaSt
     return a.dtype == GDL_DTYPE_F32 ? forward<float>(a, (float *)out, lse, st) : forward<uint16_t>(a, (uint16_t *)out, lse, st);
 }
 
-size_t attention_backward_simt_workspace(const gdl_attention &a) { return sink_bytes(a, kRows, kSinkChunk); }
-
 int attention_backward_simt(const gdl_attention &a, const void *out, const float *lse, const void *rest, const void *dout,
-                            void *dq, void *dk, void *dv, float *delta, float *part, float *sink_ws, cudaStream_t st) {
+                            void *dq, void *dk, void *dv, float *delta, float *part, float *sink_ws, int chunk,
+                            cudaStream_t st) {
     if (a.dtype == GDL_DTYPE_F32)
-        return backward<float>(a, (const float *)out, lse, (const float *)nullptr, (const float *)dout, (float *)dq, (float *)dk, (float *)dv, delta, part, sink_ws, st);
+        return backward<float>(a, (const float *)out, lse, (const float *)nullptr, (const float *)dout, (float *)dq, (float *)dk, (float *)dv, delta, part, sink_ws, chunk, st);
     return backward<uint16_t>(a, (const uint16_t *)out, lse, (const uint16_t *)rest, (const uint16_t *)dout, (uint16_t *)dq, (uint16_t *)dk, (uint16_t *)dv,
-                              delta, part, sink_ws, st);
+                              delta, part, sink_ws, chunk, st);
 }
 
 }  // namespace gdl

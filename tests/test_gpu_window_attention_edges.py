@@ -204,3 +204,11 @@ def test_nothing_is_kept_without_gradients():
         out = window_attention(q, c["k"], c["v"], c["ptr_q"], window=(4, 4))
     assert not out.requires_grad and out.grad_fn is None
     assert torch.equal(out, window_attention(q, c["k"], c["v"], c["ptr_q"], window=(4, 4)))
+
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("sinks", [130, 500])
+def test_many_sinks_of_many_clouds(dt, sinks):
+    """More sinks than a tile of keys, than a chunk of queries, and than most clouds have rows."""
+    verify(make(46, [1500, 3, 0, 140, 64, 700, 1], 2, 1, 32, DT[dt], buckets=8), (16, 16), sinks)

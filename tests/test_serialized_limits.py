@@ -1,6 +1,7 @@
 """Limits of the serialised-cloud operators that show without a GPU: refusals before a launch, workspace sizes,
 extreme arguments."""
 
+import numpy as np
 import pytest
 import torch
 
@@ -52,3 +53,43 @@ def test_few_rows_of_many_clouds_are_given_a_workspace(lib):  # noqa: F811
     assert lib.gdl_gated_scan_workspace_size(256, 65533, 8) == 256
     assert lib.gdl_gated_scan_workspace_size(256, 65534, 8) > 65534 * 8 * 4
     assert lib.gdl_gated_scan_workspace_size(0, 70000, 8) > 70000 * 8 * 4
+
+
+def test_the_workspace_of_many_sinks_is_bounded(lib):  # noqa: F811
+    """Partial sums of the sinks: what the kernels that run need, and no more than three times dK and dV in f32."""
+    def size(dtype=1, **over):
+        a = attention(dtype=dtype, heads=4, kv_heads=4, dim=64, q_row=256, k_row=256, v_row=256, q_head=64, k_head=64, v_head=64, **over)
+        return lib.gdl_window_attention_backward_workspace_size(a)
+
+    rows = dict(n_query=131072, n_key=131072, num_clouds=1, left=256, right=256)
+    plain = size(**rows)
+    grads = 131072 * 4 * 64 * 2 * 4
+    assert size(num_sinks=2048, **rows) - plain < 1.1 * grads       # 0.27 GB (chunks of 1024 queries: 0.54)
+    assert size(num_sinks=4, **rows) - plain < 0.01 * grads         # chunks of 1024: 129 of 4 rows
+    for sinks in (1, 60, 500, 10_000, 131_000, 131_072, 2 ** 31 - 1):
+        for clouds in (1, 8, 20_000):
+            for dtype in (0, 1):
+                over = dict(rows, num_clouds=clouds)
+                assert size(dtype, num_sinks=sinks, **over) - size(dtype, **over) <= 3 * grads + 512, (sinks, clouds, dtype)
+
+
+def test_partial_sums_of_sinks_lie_apart():
+    """The kernels' places, restated: cloud b's sinks from min(b * sinks, its first key) on; chunk i of its queries
+    (first query // size + i) * sinks rows further; min(clouds * sinks, keys) rows, and (queries // size) * sinks more."""
+    rng = np.random.RandomState(0)
+    for _ in range(200):
+        clouds, sinks, size = rng.randint(1, 30), rng.randint(1, 200), int(rng.choice([1, 7, 128]))
+        nk, nq = (np.where(rng.rand(clouds) < 0.2, 0, rng.randint(0, 400, clouds)) for _ in range(2))
+        k0, q0 = (np.cumsum(n) - n + rng.randint(0, 9) for n in (nk, nq))
+        n_key, n_query = int(k0[-1] + nk[-1] + rng.randint(0, 9)), int(q0[-1] + nq[-1] + rng.randint(0, 9))
+        most = min(clouds * sinks, n_key)
+        main, chunk = np.zeros(most, int), np.zeros(n_query // size * sinks + most, int)
+        for b in range(clouds):
+            base, own = min(b * sinks, int(k0[b])), min(sinks, int(nk[b]))
+            main[base:base + own] += 1
+            assert base + own <= len(main)
+            for i in range((int(nq[b]) + size - 1) // size):
+                at = (int(q0[b]) // size + i) * sinks + base
+                chunk[at:at + own] += 1
+                assert at + own <= len(chunk)
+        assert main.max(initial=0) <= 1 and chunk.max(initial=0) <= 1
