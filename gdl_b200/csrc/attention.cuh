@@ -11,6 +11,7 @@ constexpr int kAttnMaxDim = 128;
 constexpr int kAttnMaxBuckets = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kFloatMax = 3.4028234664e38f;
 
 __device__ __forceinline__ float ex2(float x) {
     float r;
@@ -64,6 +65,12 @@ __device__ __forceinline__ float bias_at(const gdl_attention &a, int64_t i) {
                                          : bf16_bits_to_f32(__ldg((const uint16_t *)a.bias + i));
 }
 
+// The same in powers of two. The type's lowest value (a mask) stays finite: a row of nothing else weighs all alike.
+__device__ __forceinline__ float bias2_at(const gdl_attention &a, int64_t i) {
+    const float b = bias_at(a, i), t = b * kLog2e;
+    return fabsf(b) <= kFloatMax ? fminf(fmaxf(t, -kFloatMax), kFloatMax) : t;
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -88,17 +95,57 @@ __device__ __forceinline__ void stage_row(float *s, const T *p, int dim) {
     for (int d = threadIdx.x & 31; d < dim; d += 32) s[d] = load1(p + d);
 }
 
-// The logit (in powers of two) of global query row qi, staged in sq, and global key row kj, head h.
+// The logit (in powers of two) of global query row qi and global key row kj, head h, from their product.
+__device__ __forceinline__ float logit2_of(const gdl_attention &a, int h, float dot, int64_t qi, int64_t kj) {
+    const float s = dot * (a.scale * kLog2e);
+    if (!a.bias) return s;
+    const float *p = a.pos_q + 3 * qi, *r = a.pos_k + 3 * kj;
+    return s + bias2_at(a, (int64_t)h * a.buckets + distance_bucket(a, p[0], p[1], p[2], r[0], r[1], r[2]));
+}
+template <typename T>
+__device__ __forceinline__ const T *key_row(const gdl_attention &a, int h, int64_t kj) {
+    return (const T *)a.k + kj * a.k_row + (int64_t)(h / (a.heads / a.kv_heads)) * a.k_head;
+}
 template <typename T>
 __device__ __forceinline__ float logit2(const gdl_attention &a, int h, const float *sq, int64_t qi, int64_t kj) {
-    const T *kp = (const T *)a.k + kj * a.k_row + (int64_t)(h / (a.heads / a.kv_heads)) * a.k_head;
-    float s = row_dot(sq, kp, a.dim) * (a.scale * kLog2e);
-    if (a.bias) {
-        const float *p = a.pos_q + 3 * qi, *r = a.pos_k + 3 * kj;
-        const int bucket = distance_bucket(a, p[0], p[1], p[2], r[0], r[1], r[2]);
-        s = fmaf(bias_at(a, (int64_t)h * a.buckets + bucket), kLog2e, s);
-    }
-    return s;
+    return logit2_of(a, h, row_dot(sq, key_row<T>(a, h, kj), a.dim), qi, kj);
+}
+
+// A row's weights in the gradients, from its logits x in powers of two: P = exp2(x + shift) inv. From the forward's
+// lse, shift is -lse and inv 1 (-inf where every logit is -inf: P = 0). Beside a large lse (a finite mask over all that a
+// row sees) 32 bits hold too little of the sum's logarithm: shift is then minus the largest logit and inv one over the sum,
+// both found anew, and x + shift is kept from rising above 0 by a rounding.
+struct RowWeight {
+    float shift, inv;
+};
+constexpr float kFarLse = 2048.0f;  // (from here on lse alone would put P off by more than 3e-4)
+__device__ __forceinline__ bool far_lse(float ls) { return fabsf(ls) > kFarLse && fabsf(ls) <= kFloatMax; }
+__device__ __forceinline__ RowWeight near_weight(float ls) {
+    return {ls == neg_inf() ? ls : ls * -kLog2e, 1.0f};
+}
+__device__ __forceinline__ float not_above_0(float x) { return x > 0.0f ? 0.0f : x; }  // (NaN stays)
+
+// One warp: the weights of a row with a large lse.
+template <typename T>
+__device__ __noinline__ RowWeight far_weight(const gdl_attention &a, int h, int64_t q0, int64_t nq, int64_t k0,
+                                             int64_t nk, int64_t row) {
+    const int lane = threadIdx.x & 31;
+    const int64_t qi = q0 + row;
+    const T *qp = (const T *)a.q + qi * a.q_row + (int64_t)h * a.q_head;
+    const KeyRange r = visible_keys(a, row + nk - nq, nk);
+    float m = neg_inf(), l = 0.0f;
+    for (int part = 0; part < 2; ++part)
+        for (int64_t j = (part ? r.lo : 0) + lane; j < (part ? r.hi : r.sinks); j += 32) {
+            const T *kp = key_row<T>(a, h, k0 + j);
+            float dot = 0.0f;
+            for (int d = 0; d < a.dim; ++d) dot = fmaf(load1(qp + d), load1(kp + d), dot);
+            const float x = logit2_of(a, h, dot, qi, k0 + j), mn = fmaxf(m, x), base = mn == neg_inf() ? 0.0f : mn;
+            l = fmaf(l, ex2(m - base), ex2(x - base));
+            m = mn;
+        }
+    const float top = warp_max(m);
+    const float sum = warp_sum(m == neg_inf() ? 0.0f : l * ex2(m - top));
+    return {-top, 1.0f / sum};
 }
 
 // One warp: output row and lse (natural) of query row `row` of a cloud (starts q0, k0; sizes nq, nk).
@@ -145,11 +192,29 @@ __device__ __noinline__ void attention_row(const gdl_attention &a, int h, int64_
     if (lse && lane == 0) lse[(int64_t)h * a.n_query + qi] = l == 0.0f ? neg_inf() : (m + log2f(l)) * kLn2;
 }
 
-// One warp: dq of a query row, delta known. sq, sd: strips of the warp's own.
+// What the dQ kernels find of each row, [3][heads][n_query]: delta, and the weights' shift and inv.
+struct RowStats {
+    float *at;
+    int64_t each;  // heads * n_query
+    __device__ __forceinline__ void put(int64_t i, float delta, RowWeight w) const {
+        at[i] = delta;
+        at[each + i] = w.shift;
+        at[2 * each + i] = w.inv;
+    }
+    __device__ __forceinline__ float delta(int64_t i) const { return at[i]; }
+    __device__ __forceinline__ float shift(int64_t i) const { return at[each + i]; }
+    __device__ __forceinline__ float inv(int64_t i) const { return at[2 * each + i]; }
+};
+__device__ __forceinline__ float weight(float x, float shift, float inv) {
+    const float e = x + shift;
+    return ex2(inv != 1.0f ? not_above_0(e) : e) * inv;
+}
+
+// One warp: dq of a query row. sq, sd: strips of the warp's own.
 template <typename T>
 __device__ __noinline__ void attention_dq_row(const gdl_attention &a, int h, int64_t q0, int64_t nq, int64_t k0,
                                               int64_t nk, int64_t row, float *sq, float *sd,
-                                              const float *lse, const float *delta, const T *dout, T *dq) {
+                                              const RowStats stats, const T *dout, T *dq) {
     const int lane = threadIdx.x & 31;
     const int64_t qi = q0 + row;
     const int hk = h / (a.heads / a.kv_heads);
@@ -158,28 +223,26 @@ __device__ __noinline__ void attention_dq_row(const gdl_attention &a, int h, int
     stage_row(sq, (const T *)a.q + qi * a.q_row + (int64_t)h * a.q_head, a.dim);
     stage_row(sd, dout + ro, a.dim);
     __syncwarp();
-    const float de = delta[(int64_t)h * a.n_query + qi], ls = lse[(int64_t)h * a.n_query + qi];
+    const int64_t at = (int64_t)h * a.n_query + qi;
+    const float de = stats.delta(at), shift = stats.shift(at), inv = stats.inv(at);
     const KeyRange r = visible_keys(a, row + nk - nq, nk);
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (ls != neg_inf()) {
-        for (int part = 0; part < 2; ++part) {
-            const int64_t from = part ? r.lo : 0, to = part ? r.hi : r.sinks;
-            for (int64_t j0 = from; j0 < to; j0 += 32) {
-                const int64_t j = j0 + lane;
-                float ds = 0.0f;
-                if (j < to) {
-                    const float p = ex2(logit2<T>(a, h, sq, qi, k0 + j) - ls * kLog2e);
-                    const T *vp = (const T *)a.v + (k0 + j) * a.v_row + (int64_t)hk * a.v_head;
-                    ds = p * (row_dot(sd, vp, a.dim) - de);
-                }
-                const int cnt = to - j0 < 32 ? (int)(to - j0) : 32;
-                for (int t = 0; t < cnt; ++t) {
-                    const float dt = __shfl_sync(0xffffffffu, ds, t);
-                    const T *kp = (const T *)a.k + (k0 + j0 + t) * a.k_row + (int64_t)hk * a.k_head;
+    for (int part = 0; part < 2; ++part) {
+        const int64_t from = part ? r.lo : 0, to = part ? r.hi : r.sinks;
+        for (int64_t j0 = from; j0 < to; j0 += 32) {
+            const int64_t j = j0 + lane;
+            float ds = 0.0f;
+            if (j < to) {
+                const T *vp = (const T *)a.v + (k0 + j) * a.v_row + (int64_t)hk * a.v_head;
+                ds = weight(logit2<T>(a, h, sq, qi, k0 + j), shift, inv) * (row_dot(sd, vp, a.dim) - de);
+            }
+            const int cnt = to - j0 < 32 ? (int)(to - j0) : 32;
+            for (int t = 0; t < cnt; ++t) {
+                const float dt = __shfl_sync(0xffffffffu, ds, t);
+                const T *kp = (const T *)a.k + (k0 + j0 + t) * a.k_row + (int64_t)hk * a.k_head;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (lane + 32 * e < a.dim) acc[e] = fmaf(dt, load1(kp + lane + 32 * e), acc[e]);
-                }
+                for (int e = 0; e < 4; ++e)
+                    if (lane + 32 * e < a.dim) acc[e] = fmaf(dt, load1(kp + lane + 32 * e), acc[e]);
             }
         }
     }
@@ -193,8 +256,7 @@ __device__ __noinline__ void attention_dq_row(const gdl_attention &a, int h, int
 template <typename T>
 __device__ __noinline__ void attention_dkv_row(const gdl_attention &a, int hk, int64_t q0, int64_t nq, int64_t k0,
                                                int64_t nk, int64_t row, int64_t lo, int64_t hi, float *sk, float *sv,
-                                               const float *lse, const float *delta, const T *dout, float *partial,
-                                               T *dk, T *dv) {
+                                               const RowStats stats, const T *dout, float *partial, T *dk, T *dv) {
     const int lane = threadIdx.x & 31;
     const int64_t kj = k0 + row;
     const int group = a.heads / a.kv_heads;
@@ -211,17 +273,10 @@ __device__ __noinline__ void attention_dkv_row(const gdl_attention &a, int hk, i
             const int64_t qi = q0 + i0 + lane;
             float p = 0.0f, ds = 0.0f;
             if (i0 + lane < r.hi) {
-                const float ls = lse[(int64_t)h * a.n_query + qi];
-                const T *qp = (const T *)a.q + qi * a.q_row + (int64_t)h * a.q_head;
-                float s = row_dot(sk, qp, a.dim) * (a.scale * kLog2e);
-                if (a.bias) {
-                    const float *x = a.pos_q + 3 * qi, *y = a.pos_k + 3 * kj;
-                    const int b = distance_bucket(a, x[0], x[1], x[2], y[0], y[1], y[2]);
-                    s = fmaf(bias_at(a, (int64_t)h * a.buckets + b), kLog2e, s);
-                }
-                p = ls == neg_inf() ? 0.0f : ex2(s - ls * kLog2e);
-                const float dp = row_dot(sv, dout + (qi * a.heads + h) * a.dim, a.dim);
-                ds = ls == neg_inf() ? 0.0f : p * (dp - delta[(int64_t)h * a.n_query + qi]);
+                const int64_t at = (int64_t)h * a.n_query + qi;
+                const float dot = row_dot(sk, (const T *)a.q + qi * a.q_row + (int64_t)h * a.q_head, a.dim);
+                p = weight(logit2_of(a, h, dot, qi, kj), stats.shift(at), stats.inv(at));
+                ds = p * (row_dot(sv, dout + (qi * a.heads + h) * a.dim, a.dim) - stats.delta(at));
             }
             const int cnt = r.hi - i0 < 32 ? (int)(r.hi - i0) : 32;
             for (int t = 0; t < cnt; ++t) {

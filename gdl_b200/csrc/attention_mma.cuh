@@ -250,9 +250,9 @@ int attention_forward_stream(const gdl_attention &a, void *out, float *lse, cuda
 int attention_simt_rows();
 int attention_forward_simt(const gdl_attention &a, void *out, float *lse, cudaStream_t st);
 int attention_backward_simt(const gdl_attention &a, const void *out, const float *lse, const void *rest, const void *dout, void *dq, void *dk,
-                            void *dv, float *delta, float *part, float *sink_ws, int chunk, cudaStream_t st);
+                            void *dv, const RowStats stats, float *part, float *sink_ws, int chunk, cudaStream_t st);
 int attention_backward_mma(const gdl_attention &a, const uint16_t *out, const float *lse, const uint16_t *rest, const uint16_t *dout,
-                           uint16_t *dq, uint16_t *dk, uint16_t *dv, float *delta, float *part, float *sink_ws,
+                           uint16_t *dq, uint16_t *dk, uint16_t *dv, const RowStats stats, float *part, float *sink_ws,
                            int chunk, cudaStream_t st);
 
 }  // namespace gdl

@@ -82,8 +82,8 @@ int reduce_bias(const gdl_attention &a, const float *part, int64_t parts, void *
 // dV of 6 ragged clouds up to 1023 rows, 4 heads of 24 over 2). By the inputs alone, as the workspace is asked for.
 int sink_chunk(const gdl_attention &a) { return takes_mma(a) ? 1024 : 128; }
 
-// workspace: delta [heads, n_query], the bucket sums of each slot of query rows, the sinks' partial sums
-size_t delta_bytes(const gdl_attention &a) { return align256((size_t)a.heads * a.n_query * 4); }
+// workspace: the rows' stats [3][heads][n_query], the bucket sums of each slot of query rows, the sinks' partial sums
+size_t stats_bytes(const gdl_attention &a) { return align256((size_t)3 * a.heads * a.n_query * 4); }
 size_t part_bytes(const gdl_attention &a) {
     return a.bias ? align256((size_t)ragged_slots(a.n_query, a.num_clouds, attention_simt_rows()) * a.heads * a.buckets * 4) : 0;
 }
@@ -112,7 +112,7 @@ extern "C" int gdl_window_attention(const gdl_attention *given, void *out, float
 extern "C" size_t gdl_window_attention_backward_workspace_size(const gdl_attention *given) {
     if (check(given) != GDL_OK) return 256;
     const gdl_attention a = normal(*given);
-    return delta_bytes(a) + part_bytes(a) + sink_bytes(a, sink_chunk(a)) + 256;
+    return stats_bytes(a) + part_bytes(a) + sink_bytes(a, sink_chunk(a)) + 256;
 }
 
 extern "C" int gdl_window_attention_backward(const gdl_attention *given, const void *out, const float *lse,
@@ -127,14 +127,15 @@ extern "C" int gdl_window_attention_backward(const gdl_attention *given, const v
     GDL_RETURN_IF(!workspace || workspace_bytes < gdl_window_attention_backward_workspace_size(given), GDL_ERR_WORKSPACE);
     cudaStream_t st = (cudaStream_t)stream;
     char *ws = (char *)workspace;
-    float *delta = (float *)ws, *part = dbias ? (float *)(ws + delta_bytes(a)) : nullptr;
-    float *sinks = (float *)(ws + delta_bytes(a) + part_bytes(a));
+    const RowStats stats = {(float *)ws, (int64_t)a.heads * a.n_query};
+    float *part = dbias ? (float *)(ws + stats_bytes(a)) : nullptr;
+    float *sinks = (float *)(ws + stats_bytes(a) + part_bytes(a));
     const uintptr_t all = (uintptr_t)out | (uintptr_t)out_rest | (uintptr_t)grad_out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
     const bool mma = takes_mma(a) && (all & 15) == 0;
     const int done = mma ? attention_backward_mma(a, (const uint16_t *)out, lse, (const uint16_t *)out_rest,
                                                   (const uint16_t *)grad_out, (uint16_t *)dq, (uint16_t *)dk,
-                                                  (uint16_t *)dv, delta, part, sinks, sink_chunk(a), st)
-                         : attention_backward_simt(a, out, lse, out_rest, grad_out, dq, dk, dv, delta, part, sinks, sink_chunk(a), st);
+                                                  (uint16_t *)dv, stats, part, sinks, sink_chunk(a), st)
+                         : attention_backward_simt(a, out, lse, out_rest, grad_out, dq, dk, dv, stats, part, sinks, sink_chunk(a), st);
     if (done != GDL_OK || !dbias) return done;
     const int64_t parts = ragged_slots(a.n_query, a.num_clouds, mma ? kMmaRows : attention_simt_rows());
     return reduce_bias(a, part, a.n_query > 0 ? parts : 0, dbias, st);

@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kFwdThreads, FwdShape<DP>::ctas)
     }
     if (BIAS)
         for (int i = tid; i < a.buckets * 32; i += kFwdThreads)
-            table[i] = bias_at(a, (int64_t)h * a.buckets + (i >> 5)) * kLog2e;
+            table[i] = bias2_at(a, (int64_t)h * a.buckets + (i >> 5));
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot;

@@ -1,6 +1,6 @@
 // window_attention_mma_bwd.cu -- gradients of the windowed attention on the tensor cores (bf16, sm_100a).
 //
-// With P = exp(s - lse) and dS = P (dO V^T - delta), delta_i = dO_i . O_i:
+// With P = exp(s - lse) (attention.cuh: RowWeight) and dS = P (dO V^T - delta), delta_i = dO_i . O_i:
 //     dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO,   dbias[b] = sum of dS over the pairs in bucket b.
 // Two kernels, each without atomics: one CTA per 128 queries streams the keys they see (dQ, delta, the
 // bucket sums); one CTA per 128 keys streams the queries that see them (dK, dV). Either recomputes S and dP;
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                        const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ CUtensorMap map_d, const uint16_t *__restrict__ out,
                        const float *__restrict__ lse, const uint16_t *__restrict__ rest, const uint16_t *__restrict__ dout, uint16_t *__restrict__ dq,
-                       float *__restrict__ delta, float *__restrict__ part) {
+                       const RowStats stats, float *__restrict__ part) {
     using S = DqShape<DP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_addr(smem_raw) & 1023);  // (through no integer: it stays a shared pointer)
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
     }
     const KeyTiles kt = key_tiles(a, t.first + nk - t.n, t.first + rows - 1 + nk - t.n, nk);
     if (t.cloud < 0 || kt.count == 0) {  // nothing to weigh: no gradient
-        for (int r = tid; r < rows; r += kBwdThreads) delta[(int64_t)h * a.n_query + row0 + r] = 0.0f;
+        for (int r = tid; r < rows; r += kBwdThreads) stats.put((int64_t)h * a.n_query + row0 + r, 0.0f, near_weight(neg_inf()));
         zero_rows(dq + (row0 * a.heads + h) * a.dim, (int64_t)a.heads * a.dim, rows, a.dim);
         if (HIST)
             for (int b = tid; b < a.buckets; b += kBwdThreads) part[(slot * a.heads + h) * a.buckets + b] = 0.0f;
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
     }
     if (BIAS) {
         for (int i = tid; i < a.buckets * 32; i += kBwdThreads)
-            table[i] = bias_at(a, (int64_t)h * a.buckets + (i >> 5)) * kLog2e;
+            table[i] = bias2_at(a, (int64_t)h * a.buckets + (i >> 5));
         if (HIST)
             for (int i = tid; i < a.buckets * kBwdSoft; i += kBwdThreads) hist[i] = 0.0f;
     }
@@ -282,9 +282,14 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
             }
             const float de = half_sum[0][r] + half_sum[1][r];
             const float ls = lse[(int64_t)h * a.n_query + qi];
-            if (pass == 0 && half == 0 && live) delta[(int64_t)h * a.n_query + qi] = ls == neg_inf() ? 0.0f : de;
-            // P = exp2(logit + shift); where every visible logit is -inf, so is the shift: P = 0, not exp2(-inf + inf)
-            const float shift = ls == neg_inf() ? ls : ls * -kLog2e;
+            RowWeight rw = near_weight(ls);
+            unsigned far = __ballot_sync(0xffffffffu, live && far_lse(ls));
+            const bool any_far = far != 0;
+            for (; far; far &= far - 1) {
+                const RowWeight f = far_weight<uint16_t>(a, h, t.start, t.n, k0, nk, t.first + (warp & 3) * 32 + __ffs(far) - 1);
+                if (lane == __ffs(far) - 1) rw = f;
+            }
+            if (pass == 0 && half == 0 && live) stats.put((int64_t)h * a.n_query + qi, ls == neg_inf() ? 0.0f : de, rw);
             bool sees_bad = false;
             for (KeyTile t_now(kt); t_now.i < kt.count && ok; t_now.next(kt), parity ^= 1, ring_k.next(), ring_v.next()) {
                 const float *kp = kpos + ring_v.at * 3 * kMmaKeys;
@@ -309,7 +314,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                     mask = t_now.mask(kCols * half, vis_lo, vis_hi, a.num_sinks);
                     cs = chunk_sets(mask);
                 }
-                const uint64_t up = pack2(shift, shift), dd = pack2(-de, -de);
+                const uint64_t up = pack2(rw.shift, rw.shift), dd = pack2(-de, -de);
 #pragma unroll
                 for (int k = 0; k < kCols / kChunk; ++k) {
                     uint32_t pk[kChunk / 2];
@@ -336,7 +341,15 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                         for (int e = 0; e < 4; e += 2) {
                             float p0, p1;
                             unpack2(add2(x[e / 2], up), p0, p1);
+                            if (any_far) {
+                                p0 = not_above_0(p0);
+                                p1 = not_above_0(p1);
+                            }
                             unpack2(mul2(pack2(ex2(p0), ex2(p1)), add2(pair(g[c + e], g[c + e + 1]), dd)), ds[e], ds[e + 1]);
+                        }
+                        if (any_far) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) ds[e] *= rw.inv;
                         }
                         if (part_seen) {
 #pragma unroll
@@ -414,25 +427,26 @@ struct DkvShape {
     static constexpr uint32_t k = 0, v = row_bytes, q = 2 * row_bytes, d = q + stages * tile_bytes;
     static constexpr uint32_t table = d + stages * tile_bytes;
     static constexpr uint32_t s_col = 0, dp_col = 64, dk_col = 128, dv_col = 128 + DP, tmem_cols = DP == 64 ? 256 : 512;
-    static uint32_t smem(int buckets) { return table + 1024 + 2 * buckets * 128 + 2 * 5 * kMmaKeys * 4 + 256; }
+    static uint32_t smem(int buckets) { return table + 1024 + 2 * buckets * 128 + 2 * 6 * kMmaKeys * 4 + 256; }
 };
 
 template <int DP, bool BIAS>
 __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
     attn_dkv_mma_kernel(const __grid_constant__ gdl_attention a, const __grid_constant__ CUtensorMap map_q,
                         const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                        const __grid_constant__ CUtensorMap map_d, const float *__restrict__ lse,
-                        const float *__restrict__ delta, uint16_t *__restrict__ dk, uint16_t *__restrict__ dv,
+                        const __grid_constant__ CUtensorMap map_d, const RowStats stats,
+                        uint16_t *__restrict__ dk, uint16_t *__restrict__ dv,
                         const SinkPlan sp, int64_t main_ctas) {
     using S = DkvShape<DP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_addr(smem_raw) & 1023);  // (through no integer: it stays a shared pointer)
     float *table = (float *)(smem + S::table);          // [2][buckets][32], of two heads in turn
-    float *cols = table + (BIAS ? 2 * a.buckets : 0) * 32;  // [2][5][64]: x, y, z, -lse (in powers of two), -delta of a tile's queries
-    uint64_t *bars = (uint64_t *)(cols + 2 * 5 * kMmaKeys);
+    float *cols = table + (BIAS ? 2 * a.buckets : 0) * 32;  // [2][6][64]: x, y, z, shift, -delta, inv of a tile's queries
+    uint64_t *bars = (uint64_t *)(cols + 2 * 6 * kMmaKeys);
     __shared__ uint32_t tmem_slot;
     __shared__ int dead, redo;
     __shared__ uint32_t bad_rows[2][6];
+    __shared__ int far_tile[2];  // some query's inv is not 1
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = a.heads / a.kv_heads;
@@ -519,7 +533,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                 }
                 // A tile's columns (two queries to a lane) and, with a new head, its table: read a step before they
                 // are written, two tiles ahead of their use.
-                float val[2][5];
+                float val[2][6];
                 int read_c = 0, read_h = hk * group;
                 const float *pos_g = a.pos_q + 3 * q0;
                 auto read_cols = [&]() {
@@ -527,24 +541,26 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                     for (int e = 0; e < 2; ++e) {
                         const int64_t qc = lo + (int64_t)read_c * kMmaKeys + lane + 32 * e, qi = qc < nq ? qc : nq - 1;
                         const int64_t at = (int64_t)read_h * a.n_query + q0 + qi;
-                        const float ls = lse[at];
-                        val[e][3] = ls == neg_inf() ? ls : ls * -kLog2e;  // (as in dQ)
-                        val[e][4] = -delta[at];
+                        val[e][3] = stats.shift(at);
+                        val[e][4] = -stats.delta(at);
+                        val[e][5] = stats.inv(at);
                         if (BIAS)
 #pragma unroll
                             for (int x = 0; x < 3; ++x) val[e][x] = pos_g[3 * qi + x];
                     }
                 };
                 auto write_cols = [&]() {
-                    float *w = cols + fill_col.at * 5 * kMmaKeys + lane;
+                    float *w = cols + fill_col.at * 6 * kMmaKeys + lane;
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int x = BIAS ? 0 : 3; x < 5; ++x) w[x * kMmaKeys + 32 * e] = val[e][x];
+                        for (int x = BIAS ? 0 : 3; x < 6; ++x) w[x * kMmaKeys + 32 * e] = val[e][x];
+                    const bool far = __any_sync(0xffffffffu, val[0][5] != 1.0f || val[1][5] != 1.0f);
+                    if (lane == 0) far_tile[fill_col.at] = far;
                     if (BIAS && read_c == 0) {
                         float *tw = table + (read_h & 1) * a.buckets * 32 + lane;
 #pragma unroll 4
-                        for (int e = 0; e < a.buckets; ++e) tw[e * 32] = bias_at(a, (int64_t)read_h * a.buckets + e) * kLog2e;
+                        for (int e = 0; e < a.buckets; ++e) tw[e * 32] = bias2_at(a, (int64_t)read_h * a.buckets + e);
                     }
                     mbar_arrive(bar_col + 8 * fill_col.at);
                     fill_col.next();
@@ -647,7 +663,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
             const uint32_t tab0 = BIAS ? rb.tab : 0;
             bool ok = true, sees_bad = false;
             for (int i = 0; i < count && ok; ++i, parity ^= 1, ring.next(), ring_col.next()) {
-                const float *cp = cols + ring_col.at * 5 * kMmaKeys;
+                const float *cp = cols + ring_col.at * 6 * kMmaKeys;
                 if (BIAS) rb.tab = tab0 + (head & 1) * a.buckets * 128;
                 ok = mbar_wait(bar_col + 8 * ring_col.at, ring_col.parity) && mbar_wait(bar_s + 8 * half, parity);
                 ok = __all_sync(0xffffffffu, ok);
@@ -667,6 +683,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                         sees_bad |= ((w ? bq.y | bd.y : bq.x | bd.x) & bits_below(vis_hi - c0 - 32 * w) &
                                      ~bits_below(vis_lo - c0 - 32 * w)) != 0;
                 }
+                const bool far = *(volatile int *)&far_tile[ring_col.at] != 0;
                 unsigned mask = 0xffffffffu;
                 ChunkSets cs = {3, 3};
                 if (c0 < all_lo || c0 + kMmaKeys > all_hi) {
@@ -707,8 +724,14 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
 #pragma unroll
                             for (int e = 0; e < 4; e += 2) {
                                 unpack2(add2(x[e / 2], e ? ls.y : ls.x), p[e], p[e + 1]);
-                                p[e] = ex2(p[e]);
-                                p[e + 1] = ex2(p[e + 1]);
+                                if (far) {
+                                    const float i0 = cp[5 * kMmaKeys + cc + e], i1 = cp[5 * kMmaKeys + cc + e + 1];
+                                    p[e] = ex2(i0 != 1.0f ? not_above_0(p[e]) : p[e]) * i0;
+                                    p[e + 1] = ex2(i1 != 1.0f ? not_above_0(p[e + 1]) : p[e + 1]) * i1;
+                                } else {
+                                    p[e] = ex2(p[e]);
+                                    p[e + 1] = ex2(p[e + 1]);
+                                }
                                 unpack2(mul2(pack2(p[e], p[e + 1]), add2(pair(g[c + e], g[c + e + 1]), e ? de.y : de.x)),
                                         q[e], q[e + 1]);
                             }
@@ -779,10 +802,10 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
 
 }  // namespace
 
-// delta [heads, n_query]; part: the bucket sums of each slot of 128 query rows (nullable); sink_ws: the partial sums of
+// stats of each row; part: the bucket sums of each slot of 128 query rows (nullable); sink_ws: the partial sums of
 // chunks of `chunk` queries
 int attention_backward_mma(const gdl_attention &a, const uint16_t *out, const float *lse, const uint16_t *rest,
-                           const uint16_t *dout, uint16_t *dq, uint16_t *dk, uint16_t *dv, float *delta, float *part, float *sink_ws,
+                           const uint16_t *dout, uint16_t *dq, uint16_t *dk, uint16_t *dv, const RowStats stats, float *part, float *sink_ws,
                            int chunk, cudaStream_t st) {
     const int nb = a.bias ? a.buckets : 0;
     const int64_t dh = a.dim, dr = (int64_t)a.heads * a.dim;
@@ -799,7 +822,7 @@ int attention_backward_mma(const gdl_attention &a, const uint16_t *out, const fl
     GDL_RETURN_IF(q_ctas > top || k_ctas + s_ctas > top, GDL_ERR_OVERFLOW);
     auto go_q = [&](auto kernel, uint32_t smem) -> int {
         GDL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        kernel<<<(unsigned)q_ctas, kBwdThreads, smem, st>>>(a, mq, mk, mv, md, out, lse, rest, dout, dq, delta, part);
+        kernel<<<(unsigned)q_ctas, kBwdThreads, smem, st>>>(a, mq, mk, mv, md, out, lse, rest, dout, dq, stats, part);
         GDL_CUDA_TRY(cudaGetLastError());
         return GDL_OK;
     };
@@ -820,7 +843,7 @@ int attention_backward_mma(const gdl_attention &a, const uint16_t *out, const fl
         return GDL_ERR_CUDA;
     auto go_k = [&](auto kernel, uint32_t smem) -> int {
         GDL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        kernel<<<(unsigned)(k_ctas + s_ctas), kBwdThreads, smem, st>>>(a, mq, mk, mv, md, lse, delta, dk, dv, sp, k_ctas);
+        kernel<<<(unsigned)(k_ctas + s_ctas), kBwdThreads, smem, st>>>(a, mq, mk, mv, md, stats, dk, dv, sp, k_ctas);
         GDL_CUDA_TRY(cudaGetLastError());
         return GDL_OK;
     };

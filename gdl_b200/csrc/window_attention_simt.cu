@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const __grid_consta
     __syncthreads();
     load_rows<T, D>((const T *)a.q + row0 * a.q_row + (int64_t)h * a.q_head, a.q_row, rows, a.dim, Q, again);
     if (a.bias)
-        for (int i = tid; i < a.buckets; i += kThreads) table[i] = bias_at(a, (int64_t)h * a.buckets + i) * kLog2e;
+        for (int i = tid; i < a.buckets; i += kThreads) table[i] = bias2_at(a, (int64_t)h * a.buckets + i);
     int vis_lo[4], vis_hi[4];  // places within a cloud fit 32 bits
     float m[4], l[4], o[4][D / 8], px[4], py[4], pz[4];
     bool seen_bad[4];
@@ -279,14 +279,15 @@ constexpr size_t dq_smem(int nb, bool hist) {
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads)
     attn_simt_dq_kernel(const __grid_constant__ gdl_attention a, const T *__restrict__ out, const float *__restrict__ lse,
-                        const T *__restrict__ rest, const T *__restrict__ dout, T *__restrict__ dq, float *__restrict__ delta,
+                        const T *__restrict__ rest, const T *__restrict__ dout, T *__restrict__ dq, const RowStats stats,
                         float *__restrict__ part) {
     extern __shared__ __align__(16) float sm[];
     float *Q = sm, *G = Q + D * kRowLd, *K = G + D * kRowLd, *V = K + D * kColLd, *Kr = V + D * kColLd,
           *P = Kr + kCols * (D + 4), *table = P + kCols * kRowLd, *hist = table + (a.bias ? a.buckets : 0);
     __shared__ uint32_t bad;
     __shared__ uint32_t again[2];
-    __shared__ float row_delta[kRows], pos[3 * kCols];
+    __shared__ float row_delta[kRows], row_shift[kRows], row_inv[kRows], pos[3 * kCols];
+    __shared__ int far;  // some row's inv is not 1
     const int tid = threadIdx.x, ty = tid >> 3, tx = tid & 7, h = blockIdx.y, hk = h / (a.heads / a.kv_heads);
     const int lane = tid & 31, warp = tid >> 5;
     const Tile t = ragged_tile(a.ptr_q, a.num_clouds, a.n_query, kRows, blockIdx.x);
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t row0 = t.start + t.first;
     if (t.cloud < 0) {
         for (int i = tid; i < rows * a.dim; i += kThreads) store1(dq + ((row0 + i / a.dim) * a.heads + h) * a.dim + i % a.dim, 0.0f);
-        for (int r = tid; r < rows; r += kThreads) delta[(int64_t)h * a.n_query + row0 + r] = 0.0f;
+        for (int r = tid; r < rows; r += kThreads) stats.put((int64_t)h * a.n_query + row0 + r, 0.0f, near_weight(neg_inf()));
         if (part)
             for (int b = tid; b < a.buckets; b += kThreads) part[((int64_t)blockIdx.x * a.heads + h) * a.buckets + b] = 0.0f;
         return;
@@ -303,6 +304,7 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t k1 = ragged_bound(a.ptr_k, a.num_clouds, a.n_key, t.cloud + 2), nk = k1 > k0 ? k1 - k0 : 0;
     const int64_t off = nk - t.n, ro = (int64_t)a.heads * a.dim;
     if (tid < 2) again[tid] = 0;
+    if (tid == 0) far = 0;
     __syncthreads();
     load_rows<T, D>((const T *)a.q + row0 * a.q_row + (int64_t)h * a.q_head, a.q_row, rows, a.dim, Q, again);
     load_rows<T, D>(dout + row0 * ro + (int64_t)h * a.dim, ro, rows, a.dim, G, again);
@@ -313,19 +315,24 @@ __global__ void __launch_bounds__(kThreads)
             s = fmaf(load1(out + at) + (rest ? load1(rest + at) : 0.0f), load1(dout + at), s);
         }
         s = warp_sum(s);
+        const float ls = lse[(int64_t)h * a.n_query + row0 + r];
+        const RowWeight w = far_lse(ls) ? far_weight<T>(a, h, t.start, t.n, k0, nk, t.first + r) : near_weight(ls);
         if (lane == 0) {
             row_delta[r] = s;
-            delta[(int64_t)h * a.n_query + row0 + r] = s;
+            row_shift[r] = w.shift;
+            row_inv[r] = w.inv;
+            if (w.inv != 1.0f) far = 1;
+            stats.put((int64_t)h * a.n_query + row0 + r, s, w);
         }
     }
     if (a.bias) {
-        for (int i = tid; i < a.buckets; i += kThreads) table[i] = bias_at(a, (int64_t)h * a.buckets + i) * kLog2e;
+        for (int i = tid; i < a.buckets; i += kThreads) table[i] = bias2_at(a, (int64_t)h * a.buckets + i);
         if (part)
             for (int i = 0; i < a.buckets; ++i) hist[i * kThreads + tid] = 0.0f;
     }
     __syncthreads();
     int vis_lo[4], vis_hi[4];
-    float ls[4], de[4], o[4][D / 8], px[4], py[4], pz[4];
+    float sh[4], de[4], o[4][D / 8], px[4], py[4], pz[4];
     bool seen_bad[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -333,7 +340,7 @@ __global__ void __launch_bounds__(kThreads)
         const KeyRange vis = visible_keys(a, t.first + r + off, nk);
         vis_lo[i] = (int)vis.lo;
         vis_hi[i] = ty * 4 + i < rows ? (int)vis.hi : 0;
-        ls[i] = lse[(int64_t)h * a.n_query + row0 + r] * kLog2e;
+        sh[i] = row_shift[r];
         de[i] = row_delta[r];
         seen_bad[i] = false;
         px[i] = py[i] = pz[i] = 0.0f;
@@ -389,10 +396,15 @@ __global__ void __launch_bounds__(kThreads)
                     b = distance_bucket(a, px[i], py[i], pz[i], pos[c], pos[kCols + c], pos[2 * kCols + c]);
                     v += table[b];
                 }
-                x[i][j] = see && ls[i] != neg_inf() ? ex2(v - ls[i]) * (g[i][j] - de[i]) : 0.0f;
+                float e = v + sh[i], f = g[i][j] - de[i];
+                if (far) {
+                    e = row_inv[ty * 4 + i] != 1.0f ? not_above_0(e) : e;
+                    f *= row_inv[ty * 4 + i];
+                }
+                x[i][j] = see ? ex2(e) * f : 0.0f;
                 // For the bucket sums alone (dQ of the row is computed again): a key that is not finite leaves lse and delta
                 // finite only with weight 0.
-                if (odd && ls[i] != neg_inf()) x[i][j] = (ls[i] - ls[i]) + (de[i] - de[i]);
+                if (odd) x[i][j] = sh[i] == neg_inf() ? 0.0f : (sh[i] - sh[i]) + (de[i] - de[i]);
                 if (part) hist[b * kThreads + tid] += x[i][j];
             }
 #pragma unroll
@@ -418,7 +430,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int r = warp; r < rows; r += kThreads / 32)
         if (again[r >> 5] >> (r & 31) & 1)
             attention_dq_row<T>(a, h, t.start, t.n, k0, nk, t.first + r, P + warp * 2 * kAttnMaxDim,
-                                P + (warp * 2 + 1) * kAttnMaxDim, lse, delta, dout, dq);
+                                P + (warp * 2 + 1) * kAttnMaxDim, stats, dout, dq);
     if (part)
         for (int b = warp; b < a.buckets; b += kThreads / 32) {
             float s = 0.0f;
@@ -430,18 +442,17 @@ __global__ void __launch_bounds__(kThreads)
 
 template <int D>
 constexpr size_t dkv_smem(int nb) {
-    return (size_t)(2 * D * kRowLd + 2 * D * kColLd + 2 * kCols * (D + 4) + 2 * kCols * kRowLd + nb + 5 * kCols) * 4;
+    return (size_t)(2 * D * kRowLd + 2 * D * kColLd + 2 * kCols * (D + 4) + 2 * kCols * kRowLd + nb + 6 * kCols) * 4;
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads)
-    attn_simt_dkv_kernel(const __grid_constant__ gdl_attention a, const float *__restrict__ lse,
-                         const float *__restrict__ delta, const T *__restrict__ dout, T *__restrict__ dk,
-                         T *__restrict__ dv, const SinkPlan sp, int64_t main_ctas) {
+    attn_simt_dkv_kernel(const __grid_constant__ gdl_attention a, const RowStats stats, const T *__restrict__ dout,
+                         T *__restrict__ dk, T *__restrict__ dv, const SinkPlan sp, int64_t main_ctas) {
     extern __shared__ __align__(16) float sm[];
     float *K = sm, *V = K + D * kRowLd, *Q = V + D * kRowLd, *G = Q + D * kColLd, *Qr = G + D * kColLd,
           *Gr = Qr + kCols * (D + 4), *P = Gr + kCols * (D + 4), *S = P + kCols * kRowLd, *cols = S + kCols * kRowLd,
-          *table = cols + 5 * kCols;
+          *table = cols + 6 * kCols;  // cols [6][kCols]: shift, delta, x, y, z, inv of a tile's queries
     __shared__ uint32_t bad;
     __shared__ uint32_t again[2];
     const int tid = threadIdx.x, ty = tid >> 3, tx = tid & 7, warp = tid >> 5;
@@ -483,15 +494,16 @@ __global__ void __launch_bounds__(kThreads)
     }
     const float scale2 = a.scale * kLog2e;
     Load<T, D> lq, lg;
-    float lc[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    float lc[6] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     auto read = [&](int h, int64_t c0) {
         const int n = (int)(u.hi - c0 < kCols ? u.hi - c0 : kCols);
         lq.read((const T *)a.q + (u.q0 + c0) * a.q_row + (int64_t)h * a.q_head, a.q_row, n, a.dim);
         lg.read(dout + (u.q0 + c0) * ro + (int64_t)h * a.dim, ro, n, a.dim);
         if (tid < kCols) {
             const int64_t q = u.q0 + c0 + (tid < n ? tid : 0), at = (int64_t)h * a.n_query + q;
-            lc[0] = lse[at] * kLog2e;
-            lc[1] = delta[at];
+            lc[0] = stats.shift(at);
+            lc[1] = stats.delta(at);
+            lc[5] = stats.inv(at);
             if (a.bias)
 #pragma unroll
                 for (int x = 0; x < 3; ++x) lc[2 + x] = a.pos_q[3 * q + x];
@@ -504,14 +516,14 @@ __global__ void __launch_bounds__(kThreads)
             __syncthreads();
             if (tid == 0) bad = 0;
             if (a.bias && c0 == u.lo)
-                for (int i = tid; i < a.buckets; i += kThreads) table[i] = bias_at(a, (int64_t)h * a.buckets + i) * kLog2e;
+                for (int i = tid; i < a.buckets; i += kThreads) table[i] = bias2_at(a, (int64_t)h * a.buckets + i);
             __syncthreads();
             if (!kAhead<D>) read(h, c0);
             lq.write(Q, kColLd, Qr, &bad);
             lg.write(G, kColLd, Gr, &bad);
             if (tid < kCols)
 #pragma unroll
-                for (int x = 0; x < 5; ++x) cols[x * kCols + tid] = lc[x];
+                for (int x = 0; x < 6; ++x) cols[x * kCols + tid] = lc[x];
             if (kAhead<D>) {
                 const bool more = c0 + kCols < u.hi;
                 if (more || h + 1 < (hk + 1) * group) read(more ? h : h + 1, more ? c0 + kCols : u.lo);
@@ -534,9 +546,9 @@ __global__ void __launch_bounds__(kThreads)
                     float v = x[i][j] * scale2;
                     if (a.bias && see)
                         v += table[distance_bucket(a, px[i], py[i], pz[i], cols[2 * kCols + c], cols[3 * kCols + c], cols[4 * kCols + c])];
-                    const float p = see && cols[c] != neg_inf() ? ex2(v - cols[c]) : 0.0f;
+                    const float p = see ? weight(v, cols[c], cols[5 * kCols + c]) : 0.0f;
                     x[i][j] = p;
-                    g[i][j] = see && cols[c] != neg_inf() ? p * (g[i][j] - cols[kCols + c]) : 0.0f;
+                    g[i][j] = see ? p * (g[i][j] - cols[kCols + c]) : 0.0f;
                 }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -574,7 +586,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int r = warp; r < rows; r += kThreads / 32)
         if (again[r >> 5] >> (r & 31) & 1)
             attention_dkv_row<T>(a, hk, u.q0, u.nq, u.k0, u.nk, u.j0 + r, u.lo, u.hi, P + warp * 2 * kAttnMaxDim,
-                                 P + (warp * 2 + 1) * kAttnMaxDim, lse, delta, dout,
+                                 P + (warp * 2 + 1) * kAttnMaxDim, stats, dout,
                                  r < u.first_out ? u.partial + (int64_t)r * 2 * a.dim : nullptr, dk, dv);
 }
 
@@ -598,7 +610,7 @@ int forward(const gdl_attention &a, T *out, float *lse, cudaStream_t st) {
 }
 
 template <typename T>
-int backward(const gdl_attention &a, const T *out, const float *lse, const T *rest, const T *dout, T *dq, T *dk, T *dv, float *delta,
+int backward(const gdl_attention &a, const T *out, const float *lse, const T *rest, const T *dout, T *dq, T *dk, T *dv, const RowStats stats,
              float *part, float *sink_ws, int chunk, cudaStream_t st) {
     const SinkPlan sp = sink_plan(a, sink_ws, kRows, chunk);
     return by_dim(a.dim, [&](auto d) -> int {
@@ -608,7 +620,7 @@ int backward(const gdl_attention &a, const T *out, const float *lse, const T *re
             const size_t smem = dq_smem<D>(nb, part != nullptr);
             GDL_CUDA_TRY(cudaFuncSetAttribute(attn_simt_dq_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             attn_simt_dq_kernel<T, D><<<dim3((unsigned)ragged_slots(a.n_query, a.num_clouds, kRows), a.heads), kThreads, smem, st>>>(
-                a, out, lse, rest, dout, dq, delta, part);
+                a, out, lse, rest, dout, dq, stats, part);
             GDL_CUDA_TRY(cudaGetLastError());
         }
         if (a.n_key > 0) {
@@ -616,7 +628,7 @@ int backward(const gdl_attention &a, const T *out, const float *lse, const T *re
             const int64_t main = ragged_slots(a.n_key, a.num_clouds, kRows) * a.kv_heads, all = main + sp.tiles * sp.slots * a.kv_heads;
             GDL_RETURN_IF(all > ((int64_t)1 << 31) - 1, GDL_ERR_OVERFLOW);
             GDL_CUDA_TRY(cudaFuncSetAttribute(attn_simt_dkv_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            attn_simt_dkv_kernel<T, D><<<(unsigned)all, kThreads, smem, st>>>(a, lse, delta, dout, dk, dv, sp, main);
+            attn_simt_dkv_kernel<T, D><<<(unsigned)all, kThreads, smem, st>>>(a, stats, dout, dk, dv, sp, main);
             GDL_CUDA_TRY(cudaGetLastError());
         }
         return join_sinks<T>(a, sp, kRows, dk, dv, st);
@@ -632,12 +644,12 @@ int attention_forward_simt(const gdl_attention &a, void *out, float *lse, cudaSt
 }
 
 int attention_backward_simt(const gdl_attention &a, const void *out, const float *lse, const void *rest, const void *dout,
-                            void *dq, void *dk, void *dv, float *delta, float *part, float *sink_ws, int chunk,
+                            void *dq, void *dk, void *dv, const RowStats stats, float *part, float *sink_ws, int chunk,
                             cudaStream_t st) {
     if (a.dtype == GDL_DTYPE_F32)
-        return backward<float>(a, (const float *)out, lse, (const float *)nullptr, (const float *)dout, (float *)dq, (float *)dk, (float *)dv, delta, part, sink_ws, chunk, st);
+        return backward<float>(a, (const float *)out, lse, (const float *)nullptr, (const float *)dout, (float *)dq, (float *)dk, (float *)dv, stats, part, sink_ws, chunk, st);
     return backward<uint16_t>(a, (const uint16_t *)out, lse, (const uint16_t *)rest, (const uint16_t *)dout, (uint16_t *)dq, (uint16_t *)dk, (uint16_t *)dv,
-                              delta, part, sink_ws, chunk, st);
+                              stats, part, sink_ws, chunk, st);
 }
 
 }  // namespace gdl

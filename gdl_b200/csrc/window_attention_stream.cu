@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps)
     float px = 0.0f, py = 0.0f, pz = 0.0f;
     if (a.bias) {
         for (int i = tid; i < heads * a.buckets; i += 32 * kStreamWarps)
-            table[i / a.buckets][i % a.buckets] = bias_at(a, (int64_t)h0 * a.buckets + i) * kLog2e;
+            table[i / a.buckets][i % a.buckets] = bias2_at(a, (int64_t)h0 * a.buckets + i);
         px = a.pos_q[3 * qi];
         py = a.pos_q[3 * qi + 1];
         pz = a.pos_q[3 * qi + 2];

@@ -212,3 +212,23 @@ def test_nothing_is_kept_without_gradients():
 def test_many_sinks_of_many_clouds(dt, sinks):
     """More sinks than a tile of keys, than a chunk of queries, and than most clouds have rows."""
     verify(make(46, [1500, 3, 0, 140, 64, 700, 1], 2, 1, 32, DT[dt], buckets=8), (16, 16), sinks)
+
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [20, 64, 96])
+@pytest.mark.parametrize("mask", [-1e4, -1e9, "lowest"])
+@pytest.mark.parametrize("lens_q", [None, [5, 3]])
+def test_buckets_masked_by_large_negative_values(dt, dim, mask, lens_q):
+    """A row whose keys are all masked by one finite value weighs them by what is left of their logits (by
+    nothing, equally, where 32 bits hold no more than the mask), and so do its gradients."""
+    c = make(44, [150, 40], 2, 1, dim, DT[dt], lens_q=lens_q, buckets=8)
+    value = torch.finfo(DT[dt]).min if mask == "lowest" else mask
+    c["bias"][0, :3] = c["bias"][1] = value
+    window, sinks = (4, 2), 1
+    got = call(c, window, sinks)
+    want, _ = plain(c, window, sinks, pair_buckets(c, 0.4, 4), logits32=mask != -1e4)
+    tol = bounds(c, len(c["q"]), extra=4 * 2.0 ** -23 * 1.5e4 if mask == -1e4 else 0.0)
+    for n in want:
+        assert bool(torch.isfinite(got[n]).all()), n
+        assert float((got[n].detach().cpu().double() - want[n]).abs().max()) <= tol[n], n
