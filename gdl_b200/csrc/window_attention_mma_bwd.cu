@@ -47,6 +47,50 @@ struct DqShape {
     }
 };
 
+// Four columns c .. c + 3 of a tile, one row: dS from S (s) and dP (g), and the bucket sums. `bits`: the columns that
+// the row sees, where `part` holds. FAR: some row's inv is not 1.
+template <bool BIAS, bool HIST, bool FAR>
+__device__ __forceinline__ void dq_step(const uint32_t *s, const uint32_t *g, int c, unsigned bits, bool part,
+                                        const float *kp, uint64_t scale2, const RowBias &rb, RowWeight rw, float de,
+                                        uint32_t mine, uint32_t *pk) {
+    const uint64_t up = pack2(rw.shift, rw.shift), dd = pack2(-de, -de);
+    unsigned u[4];
+    if (BIAS) buckets4(rb, kp, c, u);
+    uint64_t x[2];
+    logits4<BIAS>(s, scale2, rb, u, x[0], x[1]);
+    float ds[4];
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+        float p0, p1;
+        unpack2(add2(x[e / 2], up), p0, p1);
+        if (FAR) {
+            p0 = not_above_0(p0);
+            p1 = not_above_0(p1);
+        }
+        unpack2(mul2(pack2(ex2(p0), ex2(p1)), add2(pair(g[e], g[e + 1]), dd)), ds[e], ds[e + 1]);
+    }
+    if (FAR) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ds[e] *= rw.inv;
+    }
+    if (part) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (!(bits >> e & 1)) ds[e] = 0.0f;
+    }
+    if (HIST) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t at = mad(u[e], kBwdSoft * 4, mine);
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v + ds[e]));
+        }
+    }
+    pk[0] = pack_bf16(ds[0], ds[1]);
+    pk[1] = pack_bf16(ds[2], ds[3]);
+}
+
 template <int DP, bool BIAS, bool HIST>
 __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
     attn_dq_mma_kernel(const __grid_constant__ gdl_attention a, const __grid_constant__ CUtensorMap map_q,
@@ -314,62 +358,40 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                     mask = t_now.mask(kCols * half, vis_lo, vis_hi, a.num_sinks);
                     cs = chunk_sets(mask);
                 }
-                const uint64_t up = pack2(rw.shift, rw.shift), dd = pack2(-de, -de);
-#pragma unroll
-                for (int k = 0; k < kCols / kChunk; ++k) {
-                    uint32_t pk[kChunk / 2];
-                    if (!(cs.any >> k & 1)) {
-#pragma unroll
-                        for (int c = 0; c < kChunk / 2; ++c) pk[c] = 0;
-                        tmem_st8(tmem + lane_base + S::s_col + kCols * half + kChunk / 2 * k, pk);
-                        continue;
+                // dS goes over columns of S that this thread alone reads, and has read
+                const uint32_t ts = tmem + lane_base + S::s_col + kCols * half, tg = tmem + lane_base + S::dp_col + kCols * half;
+                if (any_far) {  // (rare: as little code as it takes)
+#pragma unroll 1
+                    for (int c = 0; c < kCols; c += 4) {
+                        uint32_t s[4], g[4], pk[2];
+                        tmem_ld4(ts + c, s);
+                        tmem_ld4(tg + c, g);
+                        wait_ld();
+                        dq_step<BIAS, HIST, true>(s, g, kCols * half + c, mask >> c, true, kp, scale2, rb, rw, de, mine, pk);
+                        tmem_st2(ts + c / 2, pk);
                     }
-                    uint32_t s[kChunk], g[kChunk];
-                    tmem_ld16(tmem + lane_base + S::s_col + kCols * half + kChunk * k, s);
-                    tmem_ld16(tmem + lane_base + S::dp_col + kCols * half + kChunk * k, g);
-                    wait_ld();
-                    const unsigned bits = mask >> (kChunk * k);
-                    const bool part_seen = !(cs.all >> k & 1);
+                } else {
 #pragma unroll
-                    for (int c = 0; c < kChunk; c += 4) {
-                        unsigned u[4];
-                        if (BIAS) buckets4(rb, kp, kCols * half + kChunk * k + c, u);
-                        uint64_t x[2];
-                        logits4<BIAS>(s + c, scale2, rb, u, x[0], x[1]);
-                        float ds[4];
+                    for (int k = 0; k < kCols / kChunk; ++k) {
+                        uint32_t pk[kChunk / 2];
+                        if (!(cs.any >> k & 1)) {
 #pragma unroll
-                        for (int e = 0; e < 4; e += 2) {
-                            float p0, p1;
-                            unpack2(add2(x[e / 2], up), p0, p1);
-                            if (any_far) {
-                                p0 = not_above_0(p0);
-                                p1 = not_above_0(p1);
-                            }
-                            unpack2(mul2(pack2(ex2(p0), ex2(p1)), add2(pair(g[c + e], g[c + e + 1]), dd)), ds[e], ds[e + 1]);
+                            for (int c = 0; c < kChunk / 2; ++c) pk[c] = 0;
+                            tmem_st8(ts + kChunk / 2 * k, pk);
+                            continue;
                         }
-                        if (any_far) {
+                        uint32_t s[kChunk], g[kChunk];
+                        tmem_ld16(ts + kChunk * k, s);
+                        tmem_ld16(tg + kChunk * k, g);
+                        wait_ld();
+                        const unsigned bits = mask >> (kChunk * k);
+                        const bool part_seen = !(cs.all >> k & 1);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) ds[e] *= rw.inv;
-                        }
-                        if (part_seen) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (!(bits >> (c + e) & 1)) ds[e] = 0.0f;
-                        }
-                        if (HIST) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t at = mad(u[e], kBwdSoft * 4, mine);
-                                float v;
-                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
-                                asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v + ds[e]));
-                            }
-                        }
-                        pk[c / 2] = pack_bf16(ds[0], ds[1]);
-                        pk[c / 2 + 1] = pack_bf16(ds[2], ds[3]);
+                        for (int c = 0; c < kChunk; c += 4)
+                            dq_step<BIAS, HIST, false>(s + c, g + c, kCols * half + kChunk * k + c, bits >> c, part_seen, kp,
+                                                       scale2, rb, rw, de, mine, pk + c / 2);
+                        tmem_st8(ts + kChunk / 2 * k, pk);
                     }
-                    // dS goes over columns of S that this thread alone reads, and has read
-                    tmem_st8(tmem + lane_base + S::s_col + kCols * half + kChunk / 2 * k, pk);
                 }
                 wait_st();
                 fence_before();
@@ -429,6 +451,42 @@ struct DkvShape {
     static constexpr uint32_t s_col = 0, dp_col = 64, dk_col = 128, dv_col = 128 + DP, tmem_cols = DP == 64 ? 256 : 512;
     static uint32_t smem(int buckets) { return table + 1024 + 2 * buckets * 128 + 2 * 6 * kMmaKeys * 4 + 256; }
 };
+
+// Four columns (queries) c .. c + 3 of a tile, one row (key): P and dS from S (s) and dP (g). FAR: some query's inv is
+// not 1.
+template <bool BIAS, bool FAR>
+__device__ __forceinline__ void dkv_step(const uint32_t *s, const uint32_t *g, int c, unsigned bits, bool part,
+                                         const float *cp, uint64_t scale2, const RowBias &rb, uint32_t *pk, uint32_t *gk) {
+    unsigned u[4];
+    if (BIAS) buckets4(rb, cp, c, u);
+    uint64_t x[2];
+    logits4<BIAS>(s, scale2, rb, u, x[0], x[1]);
+    const ulonglong2 ls = *reinterpret_cast<const ulonglong2 *>(cp + 3 * kMmaKeys + c);
+    const ulonglong2 de = *reinterpret_cast<const ulonglong2 *>(cp + 4 * kMmaKeys + c);
+    float p[4], q[4];
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+        unpack2(add2(x[e / 2], e ? ls.y : ls.x), p[e], p[e + 1]);
+        if (FAR) {
+            const float i0 = cp[5 * kMmaKeys + c + e], i1 = cp[5 * kMmaKeys + c + e + 1];
+            p[e] = ex2(i0 != 1.0f ? not_above_0(p[e]) : p[e]) * i0;
+            p[e + 1] = ex2(i1 != 1.0f ? not_above_0(p[e + 1]) : p[e + 1]) * i1;
+        } else {
+            p[e] = ex2(p[e]);
+            p[e + 1] = ex2(p[e + 1]);
+        }
+        unpack2(mul2(pack2(p[e], p[e + 1]), add2(pair(g[e], g[e + 1]), e ? de.y : de.x)), q[e], q[e + 1]);
+    }
+    if (part) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (!(bits >> e & 1)) p[e] = q[e] = 0.0f;
+    }
+    pk[0] = pack_bf16(p[0], p[1]);
+    pk[1] = pack_bf16(p[2], p[3]);
+    gk[0] = pack_bf16(q[0], q[1]);
+    gk[1] = pack_bf16(q[2], q[3]);
+}
 
 template <int DP, bool BIAS>
 __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
@@ -692,61 +750,43 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                     cs = chunk_sets(mask);
                 }
                 if (!idle_warp) {
+                    // P and dS go over columns of S and dP that this thread alone reads, and has read
+                    const uint32_t ts = tmem + lane_base + S::s_col + kCols * half, tg = tmem + lane_base + S::dp_col + kCols * half;
+                    if (far) {  // (rare: as little code as it takes)
+#pragma unroll 1
+                        for (int c = 0; c < kCols; c += 4) {
+                            uint32_t s[4], g[4], pk[2], gk[2];
+                            tmem_ld4(ts + c, s);
+                            tmem_ld4(tg + c, g);
+                            wait_ld();
+                            dkv_step<BIAS, true>(s, g, kCols * half + c, mask >> c, true, cp, scale2, rb, pk, gk);
+                            tmem_st2(ts + c / 2, pk);
+                            tmem_st2(tg + c / 2, gk);
+                        }
+                    } else {
 #pragma unroll
-                    for (int k = 0; k < kCols / kChunk; ++k) {
-                        // P and dS go over columns of S and dP that this thread alone reads, and has read
-                        const uint32_t ts = tmem + lane_base + S::s_col + kCols * half,
-                                       tg = tmem + lane_base + S::dp_col + kCols * half;
-                        uint32_t pk[kChunk / 2], gk[kChunk / 2];
-                        if (!(cs.any >> k & 1)) {
+                        for (int k = 0; k < kCols / kChunk; ++k) {
+                            uint32_t pk[kChunk / 2], gk[kChunk / 2];
+                            if (!(cs.any >> k & 1)) {
 #pragma unroll
-                            for (int c = 0; c < kChunk / 2; ++c) pk[c] = 0;
+                                for (int c = 0; c < kChunk / 2; ++c) pk[c] = 0;
+                                tmem_st8(ts + kChunk / 2 * k, pk);
+                                tmem_st8(tg + kChunk / 2 * k, pk);
+                                continue;
+                            }
+                            uint32_t s[kChunk], g[kChunk];
+                            tmem_ld16(ts + kChunk * k, s);
+                            tmem_ld16(tg + kChunk * k, g);
+                            wait_ld();
+                            const unsigned bits = mask >> (kChunk * k);
+                            const bool part_seen = !(cs.all >> k & 1);
+#pragma unroll
+                            for (int c = 0; c < kChunk; c += 4)
+                                dkv_step<BIAS, false>(s + c, g + c, kCols * half + kChunk * k + c, bits >> c, part_seen, cp,
+                                                      scale2, rb, pk + c / 2, gk + c / 2);
                             tmem_st8(ts + kChunk / 2 * k, pk);
-                            tmem_st8(tg + kChunk / 2 * k, pk);
-                            continue;
+                            tmem_st8(tg + kChunk / 2 * k, gk);
                         }
-                        uint32_t s[kChunk], g[kChunk];
-                        tmem_ld16(ts + kChunk * k, s);
-                        tmem_ld16(tg + kChunk * k, g);
-                        wait_ld();
-                        const unsigned bits = mask >> (kChunk * k);
-                        const bool part_seen = !(cs.all >> k & 1);
-#pragma unroll
-                        for (int c = 0; c < kChunk; c += 4) {
-                            const int cc = kCols * half + kChunk * k + c;
-                            unsigned u[4];
-                            if (BIAS) buckets4(rb, cp, cc, u);
-                            uint64_t x[2];
-                            logits4<BIAS>(s + c, scale2, rb, u, x[0], x[1]);
-                            const ulonglong2 ls = *reinterpret_cast<const ulonglong2 *>(cp + 3 * kMmaKeys + cc);
-                            const ulonglong2 de = *reinterpret_cast<const ulonglong2 *>(cp + 4 * kMmaKeys + cc);
-                            float p[4], q[4];
-#pragma unroll
-                            for (int e = 0; e < 4; e += 2) {
-                                unpack2(add2(x[e / 2], e ? ls.y : ls.x), p[e], p[e + 1]);
-                                if (far) {
-                                    const float i0 = cp[5 * kMmaKeys + cc + e], i1 = cp[5 * kMmaKeys + cc + e + 1];
-                                    p[e] = ex2(i0 != 1.0f ? not_above_0(p[e]) : p[e]) * i0;
-                                    p[e + 1] = ex2(i1 != 1.0f ? not_above_0(p[e + 1]) : p[e + 1]) * i1;
-                                } else {
-                                    p[e] = ex2(p[e]);
-                                    p[e + 1] = ex2(p[e + 1]);
-                                }
-                                unpack2(mul2(pack2(p[e], p[e + 1]), add2(pair(g[c + e], g[c + e + 1]), e ? de.y : de.x)),
-                                        q[e], q[e + 1]);
-                            }
-                            if (part_seen) {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    if (!(bits >> (c + e) & 1)) p[e] = q[e] = 0.0f;
-                            }
-                            pk[c / 2] = pack_bf16(p[0], p[1]);
-                            pk[c / 2 + 1] = pack_bf16(p[2], p[3]);
-                            gk[c / 2] = pack_bf16(q[0], q[1]);
-                            gk[c / 2 + 1] = pack_bf16(q[2], q[3]);
-                        }
-                        tmem_st8(ts + kChunk / 2 * k, pk);
-                        tmem_st8(tg + kChunk / 2 * k, gk);
                     }
                     wait_st();
                 }
