@@ -23,6 +23,7 @@ from typing import Optional, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native as nat
 
@@ -584,6 +585,16 @@ def once_only(what: str) -> None:
     """Called first in a backward: gradients of gradients are refused (autograd runs a backward with gradients
     enabled only to differentiate it again)."""
     _need(not torch.is_grad_enabled(), f"{what}: a second derivative (create_graph=True) is not available")
+
+
+def tracked(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether autograd has to see a call: gradients are enabled, or a tensor carries a forward-mode tangent (which
+    the autograd functions refuse). Without either a call goes past autograd, 8 to 15 us less on the host."""
+    if torch.is_grad_enabled():
+        return True
+    # (outside of any dual level, which torch counts from -1, there are no tangents to look for)
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _bounds(ptr: torch.Tensor, dev: torch.device) -> torch.Tensor:

@@ -18,9 +18,8 @@ class GatedScan(torch.autograd.Function):
     """(h, last) of gdl_gated_scan; differentiable w.r.t. x, gate, decay and h0."""
 
     @staticmethod
-    def forward(ctx, x: Tensor, gate: Tensor, decay: Tensor, h0: Optional[Tensor], ptr: Tensor, reverse: bool,
-                train: bool):
-        need = train and any(ctx.needs_input_grad[:4])
+    def forward(ctx, x: Tensor, gate: Tensor, decay: Tensor, h0: Optional[Tensor], ptr: Tensor, reverse: bool):
+        need = any(ctx.needs_input_grad[:4])
         h, last, states, held = csrc.gated_scan_cuda(x, gate, decay, ptr, h0, reverse, with_states=need)
         if need:
             ctx.save_for_backward(*held, states)
@@ -35,7 +34,7 @@ class GatedScan(torch.autograd.Function):
         x, gate, decay, ptr, states = ctx.saved_tensors
         dx, dgate, ddecay, dh0 = csrc.gated_scan_backward_cuda(x, gate, decay, ptr, states, grad_h, grad_last,
                                                                ctx.reverse, want_h0=ctx.needs_input_grad[3])
-        return dx, dgate, ddecay.to(ctx.like[0]), dh0 if dh0 is None else dh0.to(ctx.like[1]), None, None, None
+        return dx, dgate, ddecay.to(ctx.like[0]), dh0 if dh0 is None else dh0.to(ctx.like[1]), None, None
 
 
 def gated_scan(x: Tensor, gate: Tensor, decay: Tensor, ptr: Tensor, *, h0: Optional[Tensor] = None,
@@ -48,4 +47,6 @@ def gated_scan(x: Tensor, gate: Tensor, decay: Tensor, ptr: Tensor, *, h0: Optio
     an empty cloud): pass it as the next call's h0 to go on with a stream, one row or many at a time.
     ``reverse`` runs each cloud from its last row to its first. States are float32 throughout.
     Gradients w.r.t. x, gate, decay and h0; bit-reproducible."""
-    return GatedScan.apply(x, gate, decay, h0, ptr, reverse, torch.is_grad_enabled())
+    if csrc.tracked(x, gate, decay, h0):
+        return GatedScan.apply(x, gate, decay, h0, ptr, reverse)
+    return csrc.gated_scan_cuda(x, gate, decay, ptr, h0, reverse, with_states=False)[:2]

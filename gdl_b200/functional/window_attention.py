@@ -23,8 +23,8 @@ class WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q: Tensor, k: Tensor, v: Tensor, bias: Optional[Tensor], pos_q: Optional[Tensor],
-                pos_k: Optional[Tensor], meta, train: bool):
-        need = train and any(ctx.needs_input_grad[:4])
+                pos_k: Optional[Tensor], meta):
+        need = any(ctx.needs_input_grad[:4])
         out, lse, rest, args = csrc.window_attention_cuda(q, k, v, bias, *meta[:5], pos_q, pos_k, *meta[5:], with_lse=need)
         if need:
             q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k = args[0]
@@ -38,7 +38,7 @@ class WindowAttention(torch.autograd.Function):
         out, lse, rest, *held = ctx.saved_tensors
         dq, dk, dv, db = csrc.window_attention_backward_cuda(held, ctx.meta, out, lse, rest, grad_out,
                                                              want_bias=ctx.needs_input_grad[3])
-        return dq, dk, dv, db, None, None, None, None
+        return dq, dk, dv, db, None, None, None
 
 
 def window_attention(q: Tensor, k: Tensor, v: Tensor, ptr_q: Tensor, *, ptr_k: Optional[Tensor] = None,
@@ -65,4 +65,7 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, ptr_q: Tensor, *, ptr_k: O
         raise csrc.nat.GdlError("window_attention: positions are constants of the bias; detach them")
     meta = (ptr_q, ptr_q if ptr_k is None else ptr_k, window, num_sinks,
             1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None else scale, radius, steps)
-    return WindowAttention.apply(q, k, v, bias, pos_q, pos_q if pos_k is None else pos_k, meta, torch.is_grad_enabled())
+    pos_k = pos_q if pos_k is None else pos_k
+    if csrc.tracked(q, k, v, bias, pos_q, pos_k):
+        return WindowAttention.apply(q, k, v, bias, pos_q, pos_k, meta)
+    return csrc.window_attention_cuda(q, k, v, bias, *meta[:5], pos_q, pos_k, *meta[5:], with_lse=False)[0]
