@@ -612,7 +612,7 @@ def _points(p: torch.Tensor) -> torch.Tensor:
     return p if p.dtype == torch.float32 and p.is_contiguous() else p.float().contiguous()
 
 
-def _attention_args(held, meta) -> nat.Attention:
+def _attention_args(held, meta, status: Optional[torch.Tensor]) -> nat.Attention:
     q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k = held
     left, right, sinks, scale, inv_r2, steps_log2 = meta
     return nat.Attention(
@@ -621,11 +621,11 @@ def _attention_args(held, meta) -> nat.Attention:
         k.shape[1], q.shape[2], nat.DTYPE[q.dtype], sinks, left, right, scale,
         None if bias is None else bias.data_ptr(), 0 if bias is None else nat.DTYPE[bias.dtype],
         0 if bias is None else bias.shape[1], steps_log2, inv_r2, None if bias is None else pos_q.data_ptr(),
-        None if bias is None else pos_k.data_ptr(), None)
+        None if bias is None else pos_k.data_ptr(), nat.ptr(status))
 
 
 def window_attention_cuda(q, k, v, bias, ptr_q, ptr_k, window, num_sinks, scale, pos_q, pos_k, radius, steps,
-                          with_lse: bool = True):
+                          with_lse: bool = True, status: Optional[torch.Tensor] = None):
     """gdl_window_attention on checked arguments (functional.window_attention documents them). Returns
     (out, lse [H, Nq], out_rest or None (both only with ``with_lse``), what the backward needs)."""
     what = "window_attention"
@@ -642,6 +642,9 @@ def window_attention_cuda(q, k, v, bias, ptr_q, ptr_k, window, num_sinks, scale,
     left, right = int(window[0]), int(window[1])
     _need(left >= -1 and right >= -1, f"{what}: window sides are -1 (open) or at least 0")
     _need(int(num_sinks) >= 0, f"{what}: num_sinks must not be negative")
+    if status is not None:
+        _need(status.is_cuda and status.device == dev and status.dtype == torch.int32 and status.numel() >= 1,
+              f"{what}: status must be an int32 CUDA tensor of at least one element, on the rows' device")
     inv_r2, steps_log2 = 0.0, 0
     if bias is not None:
         _need(bias.dim() == 2 and bias.shape[0] == H and 1 <= bias.shape[1] <= 64 and bias.dtype in nat.DTYPE,
@@ -665,17 +668,18 @@ def window_attention_cuda(q, k, v, bias, ptr_q, ptr_k, window, num_sinks, scale,
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty(H, q.shape[0], dtype=torch.float32, device=dev) if with_lse else None
     rest = torch.empty_like(out) if with_lse and q.dtype == torch.bfloat16 else None
-    a = _attention_args(held, meta)
+    a = _attention_args(held, meta, status)
     nat.check(nat.load().gdl_window_attention(a, out.data_ptr(), nat.ptr(lse), nat.ptr(rest), nat.stream(dev)),
               "gdl_window_attention")
     return out, lse, rest, (held, meta)
 
 
-def window_attention_backward_cuda(held, meta, out, lse, rest, grad_out, want_bias: bool = True):
+def window_attention_backward_cuda(held, meta, out, lse, rest, grad_out, want_bias: bool = True,
+                                   status: Optional[torch.Tensor] = None):
     """(dq, dk, dv, dbias or None) of gdl_window_attention_backward."""
     q, k, v, bias = held[:4]
     dev = q.device
-    a = _attention_args(held, meta)
+    a = _attention_args(held, meta, status)
     if grad_out.dtype != q.dtype or not grad_out.is_contiguous():
         grad_out = grad_out.to(q.dtype).contiguous()
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))

@@ -23,13 +23,14 @@ class WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q: Tensor, k: Tensor, v: Tensor, bias: Optional[Tensor], pos_q: Optional[Tensor],
-                pos_k: Optional[Tensor], meta):
+                pos_k: Optional[Tensor], meta, status: Optional[Tensor]):
         need = any(ctx.needs_input_grad[:4])
-        out, lse, rest, args = csrc.window_attention_cuda(q, k, v, bias, *meta[:5], pos_q, pos_k, *meta[5:], with_lse=need)
+        out, lse, rest, args = csrc.window_attention_cuda(q, k, v, bias, *meta[:5], pos_q, pos_k, *meta[5:], with_lse=need,
+                                                        status=status)
         if need:
             q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k = args[0]
             ctx.save_for_backward(out, lse, rest, q, k, v, bias, ptr_q, ptr_k, pos_q, pos_k)
-            ctx.meta = args[1]
+            ctx.meta, ctx.status = args[1], status
         return out
 
     @staticmethod
@@ -37,14 +38,14 @@ class WindowAttention(torch.autograd.Function):
         csrc.once_only("window_attention")
         out, lse, rest, *held = ctx.saved_tensors
         dq, dk, dv, db = csrc.window_attention_backward_cuda(held, ctx.meta, out, lse, rest, grad_out,
-                                                             want_bias=ctx.needs_input_grad[3])
-        return dq, dk, dv, db, None, None, None
+                                                             want_bias=ctx.needs_input_grad[3], status=ctx.status)
+        return dq, dk, dv, db, None, None, None, None
 
 
 def window_attention(q: Tensor, k: Tensor, v: Tensor, ptr_q: Tensor, *, ptr_k: Optional[Tensor] = None,
                      window: Tuple[int, int] = (-1, -1), num_sinks: int = 0, scale: Optional[float] = None,
                      bias: Optional[Tensor] = None, pos_q: Optional[Tensor] = None, pos_k: Optional[Tensor] = None,
-                     radius: float = 1.0, steps: int = 4) -> Tensor:
+                     radius: float = 1.0, steps: int = 4, status: Optional[Tensor] = None) -> Tensor:
     """out [Nq, H, D]: attention of q [Nq, H, D] over k, v [Nk, Hk, D] within each cloud (H a multiple
     of Hk: heads that share keys and values), float32 or bfloat16, D <= 128.
 
@@ -60,6 +61,9 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, ptr_q: Tensor, *, ptr_k: O
                   (1, 2, 4, 8 or 16) buckets to each doubling of t, the last one open. Positions are
                   constants (no gradient).
 
+    status        int32 CUDA tensor of one element, zeroed by the caller: receives GDL_ERR_TIMEOUT (6) if a
+                  bounded wait of a kernel gave up, forward or backward (never observed; its rows are NaN).
+
     A row that sees no key gives 0. Gradients w.r.t. q, k, v and bias; bit-reproducible."""
     if (pos_q is not None and pos_q.requires_grad) or (pos_k is not None and pos_k.requires_grad):
         raise csrc.nat.GdlError("window_attention: positions are constants of the bias; detach them")
@@ -67,5 +71,5 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, ptr_q: Tensor, *, ptr_k: O
             1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None else scale, radius, steps)
     pos_k = pos_q if pos_k is None else pos_k
     if csrc.tracked(q, k, v, bias, pos_q, pos_k):
-        return WindowAttention.apply(q, k, v, bias, pos_q, pos_k, meta)
-    return csrc.window_attention_cuda(q, k, v, bias, *meta[:5], pos_q, pos_k, *meta[5:], with_lse=False)[0]
+        return WindowAttention.apply(q, k, v, bias, pos_q, pos_k, meta, status)
+    return csrc.window_attention_cuda(q, k, v, bias, *meta[:5], pos_q, pos_k, *meta[5:], with_lse=False, status=status)[0]

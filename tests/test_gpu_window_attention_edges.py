@@ -232,3 +232,12 @@ def test_buckets_masked_by_large_negative_values(dt, dim, mask, lens_q):
     for n in want:
         assert bool(torch.isfinite(got[n]).all()), n
         assert float((got[n].detach().cpu().double() - want[n]).abs().max()) <= tol[n], n
+
+
+@pytest.mark.parametrize("dim", [64, 96])
+def test_the_status_word_stays_0(dim):
+    c = make(50, [300], 2, 1, dim, torch.bfloat16)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q = c["q"].requires_grad_(True)
+    window_attention(q, c["k"], c["v"], c["ptr_q"], window=(40, 40), status=status).backward(c["dout"])
+    assert int(status) == 0 and bool(torch.isfinite(q.grad).all())

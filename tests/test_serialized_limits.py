@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from gdl_b200 import csrc
+from gdl_b200.functional import window_attention
 from gdl_b200.serialized import morton_order
 
 from .test_serialized_host import INVALID, attention, lib  # noqa: F401
@@ -93,3 +94,38 @@ def test_partial_sums_of_sinks_lie_apart():
                 chunk[at:at + own] += 1
                 assert at + own <= len(chunk)
         assert main.max(initial=0) <= 1 and chunk.max(initial=0) <= 1
+
+
+def test_the_status_word_reaches_both_directions(monkeypatch):
+    """What a bounded wait that gave up would write to is the caller's tensor, in the forward and in the backward."""
+    seen = []
+
+    class Lib:  # in the library's place: notes the status word that it is given
+        def gdl_window_attention(self, a, *rest):
+            return seen.append(a.status) or 0
+
+        def gdl_window_attention_backward_workspace_size(self, a):
+            return 256
+
+        def gdl_window_attention_backward(self, a, *rest):
+            return seen.append(a.status) or 0
+
+    monkeypatch.setattr(csrc.nat, "load", lambda: Lib())
+    monkeypatch.setattr(csrc.nat, "require_cuda", lambda *t, what: torch.device("cpu"))
+    monkeypatch.setattr(csrc.nat, "stream", lambda dev: 0)
+    monkeypatch.setattr(csrc, "_bounds", lambda p, dev: p)
+
+    class Word(torch.Tensor):
+        is_cuda = True
+
+    word = torch.zeros(1, dtype=torch.int32).as_subclass(Word)
+    x, ptr = torch.zeros(4, 2, 8, requires_grad=True), torch.tensor([0, 4])
+    for status, want in ((word, word.data_ptr()), (None, None)):
+        window_attention(x, x, x, ptr, status=status).sum().backward()
+        with torch.no_grad():
+            window_attention(x, x, x, ptr, status=status)
+        assert seen == [want] * 3
+        seen.clear()
+    for bad in (torch.zeros(1, dtype=torch.int32), torch.zeros(1).as_subclass(Word), torch.zeros(0, dtype=torch.int32).as_subclass(Word)):
+        with pytest.raises(csrc.nat.GdlError):
+            window_attention(x, x, x, ptr, status=bad)
