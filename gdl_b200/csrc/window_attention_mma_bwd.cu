@@ -691,6 +691,7 @@ __global__ void __launch_bounds__(kBwdThreads, DP == 64 ? 2 : 1)
                     ring.next();
                     parity ^= 1;
                 }
+                ring_col = fill_col;  // (all columns are written: a second pass goes on from there, as their readers do)
                 if (ok) mma_commit(bar_end, issue);
                 if (!ok) {
                     *vdead = 1;

@@ -241,3 +241,26 @@ def test_the_status_word_stays_0(dim):
     q = c["q"].requires_grad_(True)
     window_attention(q, c["k"], c["v"], c["ptr_q"], window=(40, 40), status=status).backward(c["dout"])
     assert int(status) == 0 and bool(torch.isfinite(q.grad).all())
+
+
+@pytest.mark.parametrize("dim", [64, 96])
+@pytest.mark.parametrize("heads,kv", [(1, 1), (3, 1), (2, 2)])
+@pytest.mark.parametrize("lens", [[60], [190], [300, 40]])
+@pytest.mark.parametrize("name", ["q", "k", "v", "dout"])
+def test_second_passes_over_odd_numbers_of_tiles(dim, heads, kv, lens, name):
+    """A second pass goes on where the first one left its rings of buffers, at any number of tiles (1, 3, 5 to a
+    head here): no wait runs out, and rows that see nothing of it come out as they are."""
+    c = make(51, lens, heads, kv, dim, torch.bfloat16, buckets=8)
+    window = (200, 200)
+    clean = call(c, window, 0)
+    c[name][0] = float("nan")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    leaf = {n: c[n].detach().requires_grad_(True) for n in ("q", "k", "v", "bias")}
+    out = window_attention(leaf["q"], leaf["k"], leaf["v"], c["ptr_q"], window=window, bias=leaf["bias"], pos_q=c["pos_q"],
+                           radius=0.4, status=status)
+    got = {"out": out, **dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, [leaf[n] for n in "qkv"], c["dout"])))}
+    assert int(status) == 0
+    for n in got:
+        # beyond what row 0 reaches, and in the other cloud
+        far = min(2 * window[0] + 1 if n in ("dk", "dv", "dq") else window[0] + 1, lens[0])
+        assert torch.equal(got[n][far:], clean[n][far:]), n
