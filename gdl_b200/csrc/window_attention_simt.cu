@@ -6,8 +6,8 @@
 // shared-memory reads to 16 FFMA) and 4 x (dim / 8) of the outputs. Tiles lie transposed ([dim][row]) where
 // they are summed over dim, as they are where they are summed over rows. What is not finite does not go into a
 // tile (0 times it would reach other rows): a row of the CTA that has such a value, or that sees a column (a key; in
-// the dK, dV kernel a query) with one, is computed again, by itself, from what it sees. 6 ragged clouds up to 1023 rows, 4 heads of 24 over 2, window 129, 16 buckets,
-// f32: 49 us forward, 61 us dQ, 102 us dK and dV, far from what the FFMA take: 232 CTAs of 4 warps.
+// the dK, dV kernel a query) with one, is computed again, by itself, from what it sees.
+// 6 ragged clouds up to 1023 rows, 4 heads of 24 over 2, window 129, 16 buckets, f32: 48 us forward, 62 us dQ, 94 us dK and dV, far from what the FFMA take: 232 CTAs of 4 warps.
 #include "attention_sinks.cuh"
 
 namespace gdl {

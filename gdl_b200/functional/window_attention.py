@@ -4,7 +4,8 @@ distance between the two points (no counterpart in the reference).
 The rows of a cloud lie in an order that keeps neighbours near each other (a space-filling curve, a
 sweep's scan order), so a window of rows is a neighbourhood. ``num_sinks`` first rows stay visible
 beyond the window (register rows, or farthest-point samples put in front). The bias depends on the two
-points' distance alone, so it leaves a layer invariant under rotations and shifts of the cloud.
+points' distance alone, so rotations and shifts of the cloud do not change it (they may change the order of
+the rows, and with it the windows).
 """
 
 from __future__ import annotations
@@ -64,7 +65,10 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, ptr_q: Tensor, *, ptr_k: O
     status        int32 CUDA tensor of one element, zeroed by the caller: receives GDL_ERR_TIMEOUT (6) if a
                   bounded wait of a kernel gave up, forward or backward (never observed; its rows are NaN).
 
-    A row that sees no key gives 0. Gradients w.r.t. q, k, v and bias; bit-reproducible."""
+    A row that sees no key gives 0, and so does one whose logits are all -inf (a bias may hold -inf); both take no
+    part in a gradient. What a row does not see never reaches its result; a NaN or an infinity in q, or in a key that
+    it sees, does. Logits are held in 32 bits: a row masked throughout by a large negative bias weighs its keys alike.
+    Gradients w.r.t. q, k, v and bias (of first order); bit-reproducible."""
     if (pos_q is not None and pos_q.requires_grad) or (pos_k is not None and pos_k.requires_grad):
         raise csrc.nat.GdlError("window_attention: positions are constants of the bias; detach them")
     meta = (ptr_q, ptr_q if ptr_k is None else ptr_k, window, num_sinks,

@@ -433,8 +433,10 @@ int gdl_gather_rows(const void *src, int64_t n_src, int64_t row_bytes, const int
  * what is cached. Key j is visible to it iff
  *     (right < 0 or j <= i + right) and (left < 0 or j >= i - left or j < num_sinks);
  *     s_ij = scale * q_i . k_j + bias[h, bucket(p_i, p_j)];   out_i = sum_j softmax_j(s_ij) v_j.
- * A row that sees no key gets out = 0 and lse = -inf; a query row of no cloud gets out = 0. What a
- * row does not see never reaches its result, NaN and infinities included.
+ * A row that sees no key, or whose logits are all -inf, gets out = 0 and lse = -inf, and takes no part in
+ * a gradient; a query row of no cloud gets out = 0. What a row does not see never reaches its result, NaN
+ * and infinities included. What is not finite in a row, or in what it sees, makes its result not finite as
+ * the formulas have it; a row of a gradient may then be NaN as a whole.
  * bucket(p, r): t = fma(|p - r|^2, inv_radius2, 1) in f32, bucket = min(buckets - 1,
  *     (bits(t) >> (23 - steps_log2)) - (127 << steps_log2)): 2^steps_log2 buckets to each doubling of
  *     t, the first from distance 0, the last open; rotations and shifts of a cloud do not change it.
@@ -461,8 +463,8 @@ typedef struct {
 /* out [n_query, heads, dim] contiguous; lse [heads, n_query] f32 (nullable): natural logarithm of the
  * softmax denominators, which the backward needs. out_rest (nullable; shape and type of out, bf16 only):
  * what the rounding of out to bf16 left over (0 where a kernel does not compute it). The backward takes
- * delta = grad_out . out from both: of the roundings of bf16, only P's is left in it (dbias, a sum of
- * differences against delta, is then off by 1.3 roundings of its own instead of 1.5). */
+ * delta = grad_out . out from both. It is worth little: dq is off by 0.00244 with it and by 0.00248 without
+ * (16 x 2048 points, 4 heads of 32), by 0.00239 and 0.00240 at 131072 points, dbias by as much either way. */
 int gdl_window_attention(const gdl_attention *a, void *out, float *lse, void *out_rest, void *stream);
 
 /* Gradients for grad_out, out [n_query, heads, dim] contiguous, lse and out_rest (nullable) of the forward.
