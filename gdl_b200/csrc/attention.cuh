@@ -26,6 +26,13 @@ __device__ __forceinline__ float load1(const uint16_t *p) { return bf16_bits_to_
 __device__ __forceinline__ void store1(float *p, float v) { *p = v; }
 __device__ __forceinline__ void store1(uint16_t *p, float v) { *p = f32_to_bf16_bits(v); }
 
+// v to *p, and to *rest, if given, what that left over
+template <typename T>
+__device__ __forceinline__ void store_rest(T *p, T *rest, float v) {
+    store1(p, v);
+    if (sizeof(T) == 2 && rest) store1(rest, v - bf16_bits_to_f32(f32_to_bf16_bits(v)));
+}
+
 // keys that the query at place i of a cloud of nk keys sees: [0, sinks) and [lo, hi)
 struct KeyRange {
     int64_t sinks, lo, hi;
@@ -149,10 +156,10 @@ __device__ __noinline__ RowWeight far_weight(const gdl_attention &a, int h, int6
 }
 
 // One warp: output row and lse (natural) of query row `row` of a cloud (starts q0, k0; sizes nq, nk).
-// sq: kAttnMaxDim floats of the warp's own.
+// sq: kAttnMaxDim floats of the warp's own. rest (nullable): what rounding the output left over.
 template <typename T>
 __device__ __noinline__ void attention_row(const gdl_attention &a, int h, int64_t q0, int64_t nq, int64_t k0,
-                                           int64_t nk, int64_t row, float *sq, T *out, float *lse) {
+                                           int64_t nk, int64_t row, float *sq, T *out, float *lse, T *rest) {
     const int lane = threadIdx.x & 31;
     const int64_t qi = q0 + row;
     const int hk = h / (a.heads / a.kv_heads);
@@ -188,7 +195,7 @@ __device__ __noinline__ void attention_row(const gdl_attention &a, int h, int64_
     T *op = out + (qi * a.heads + h) * a.dim;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (lane + 32 * e < a.dim) store1(op + lane + 32 * e, acc[e] * inv);
+        if (lane + 32 * e < a.dim) store_rest(op + lane + 32 * e, rest ? rest + (op - out) + lane + 32 * e : nullptr, acc[e] * inv);
     if (lse && lane == 0) lse[(int64_t)h * a.n_query + qi] = l == 0.0f ? neg_inf() : (m + log2f(l)) * kLn2;
 }
 

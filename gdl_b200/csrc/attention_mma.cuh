@@ -246,9 +246,9 @@ bool mma_layout(const void *p, int64_t head_stride, int64_t row_stride, int head
 
 int attention_forward_mma(const gdl_attention &a, uint16_t *out, float *lse, uint16_t *rest, cudaStream_t st);
 bool takes_stream(const gdl_attention &a);
-int attention_forward_stream(const gdl_attention &a, void *out, float *lse, cudaStream_t st);
+int attention_forward_stream(const gdl_attention &a, void *out, float *lse, void *rest, cudaStream_t st);
 int attention_simt_rows();
-int attention_forward_simt(const gdl_attention &a, void *out, float *lse, cudaStream_t st);
+int attention_forward_simt(const gdl_attention &a, void *out, float *lse, void *rest, cudaStream_t st);
 int attention_backward_simt(const gdl_attention &a, const void *out, const float *lse, const void *rest, const void *dout, void *dq, void *dk,
                             void *dv, const RowStats stats, float *part, float *sink_ws, int chunk, cudaStream_t st);
 int attention_backward_mma(const gdl_attention &a, const uint16_t *out, const float *lse, const uint16_t *rest, const uint16_t *dout,

@@ -104,9 +104,8 @@ extern "C" int gdl_window_attention(const gdl_attention *given, void *out, float
     const bool few = takes_stream(a);
     if (!few && takes_mma(a) && (((uintptr_t)out | (uintptr_t)out_rest) & 15) == 0)
         return attention_forward_mma(a, (uint16_t *)out, lse, (uint16_t *)out_rest, st);
-    if (out_rest) GDL_CUDA_TRY(cudaMemsetAsync(out_rest, 0, (size_t)a.n_query * a.heads * a.dim * 2, st));
-    if (few) return attention_forward_stream(a, out, lse, st);
-    return attention_forward_simt(a, out, lse, st);
+    if (few) return attention_forward_stream(a, out, lse, out_rest, st);
+    return attention_forward_simt(a, out, lse, out_rest, st);
 }
 
 extern "C" size_t gdl_window_attention_backward_workspace_size(const gdl_attention *given) {

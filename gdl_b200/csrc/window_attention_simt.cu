@@ -138,7 +138,7 @@ constexpr size_t fwd_smem(int nb) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const __grid_constant__ gdl_attention a, T *__restrict__ out,
-                                                             float *__restrict__ lse) {
+                                                             float *__restrict__ lse, T *__restrict__ rest) {
     extern __shared__ __align__(16) float sm[];
     float *Q = sm, *K = Q + D * kRowLd, *V = K + D * kColLd, *P = V + kCols * (D + 4), *table = P + kCols * kRowLd;
     __shared__ uint32_t bad;
@@ -150,7 +150,10 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const __grid_consta
     const int rows = (int)(t.n - t.first < kRows ? t.n - t.first : kRows);
     const int64_t row0 = t.start + t.first;
     if (t.cloud == -1) {
-        for (int i = tid; i < rows * a.dim; i += kThreads) store1(out + ((row0 + i / a.dim) * a.heads + h) * a.dim + i % a.dim, 0.0f);
+        for (int i = tid; i < rows * a.dim; i += kThreads) {
+            const int64_t at = ((row0 + i / a.dim) * a.heads + h) * a.dim + i % a.dim;
+            store_rest(out + at, rest ? rest + at : nullptr, 0.0f);
+        }
         if (lse)
             for (int r = tid; r < rows; r += kThreads) lse[(int64_t)h * a.n_query + row0 + r] = neg_inf();
         return;
@@ -256,19 +259,20 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const __grid_consta
         const int r = ty * 4 + i;
         if (r >= rows) continue;
         const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
-        T *op = out + ((row0 + r) * a.heads + h) * a.dim;
+        const int64_t at = ((row0 + r) * a.heads + h) * a.dim + tx * 4;
 #pragma unroll
         for (int g = 0; g < D / 32; ++g)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (tx * 4 + 32 * g + j < a.dim) store1(op + tx * 4 + 32 * g + j, o[i][4 * g + j] * inv);
+                if (tx * 4 + 32 * g + j < a.dim)
+                    store_rest(out + at + 32 * g + j, rest ? rest + at + 32 * g + j : nullptr, o[i][4 * g + j] * inv);
         if (tx == 0 && lse) lse[(int64_t)h * a.n_query + row0 + r] = l[i] == 0.0f ? neg_inf() : (m[i] + log2f(l[i])) * kLn2;
         if (seen_bad[i]) atomicOr(again + (r >> 5), 1u << (r & 31));
     }
     __syncthreads();
     for (int r = tid >> 5; r < rows; r += kThreads / 32)
         if (again[r >> 5] >> (r & 31) & 1)
-            attention_row<T>(a, h, t.start, t.n, k0, nk, t.first + r, P + (tid >> 5) * kAttnMaxDim, out, lse);
+            attention_row<T>(a, h, t.start, t.n, k0, nk, t.first + r, P + (tid >> 5) * kAttnMaxDim, out, lse, rest);
 }
 
 template <int D>
@@ -598,12 +602,12 @@ int by_dim(int dim, F f) {
 }
 
 template <typename T>
-int forward(const gdl_attention &a, T *out, float *lse, cudaStream_t st) {
+int forward(const gdl_attention &a, T *out, float *lse, T *rest, cudaStream_t st) {
     return by_dim(a.dim, [&](auto d) -> int {
         constexpr int D = decltype(d)::value;
         const size_t smem = fwd_smem<D>(a.bias ? a.buckets : 0);
         GDL_CUDA_TRY(cudaFuncSetAttribute(attn_simt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        attn_simt_kernel<T, D><<<dim3((unsigned)ragged_slots(a.n_query, a.num_clouds, kRows), a.heads), kThreads, smem, st>>>(a, out, lse);
+        attn_simt_kernel<T, D><<<dim3((unsigned)ragged_slots(a.n_query, a.num_clouds, kRows), a.heads), kThreads, smem, st>>>(a, out, lse, rest);
         GDL_CUDA_TRY(cudaGetLastError());
         return GDL_OK;
     });
@@ -639,8 +643,9 @@ int backward(const gdl_attention &a, const T *out, const float *lse, const T *re
 
 int attention_simt_rows() { return kRows; }
 
-int attention_forward_simt(const gdl_attention &a, void *out, float *lse, cudaStream_t st) {
-    return a.dtype == GDL_DTYPE_F32 ? forward<float>(a, (float *)out, lse, st) : forward<uint16_t>(a, (uint16_t *)out, lse, st);
+int attention_forward_simt(const gdl_attention &a, void *out, float *lse, void *rest, cudaStream_t st) {
+    return a.dtype == GDL_DTYPE_F32 ? forward<float>(a, (float *)out, lse, nullptr, st)
+                                    : forward<uint16_t>(a, (uint16_t *)out, lse, (uint16_t *)rest, st);
 }
 
 int attention_backward_simt(const gdl_attention &a, const void *out, const float *lse, const void *rest, const void *dout,

@@ -59,7 +59,8 @@ __device__ __forceinline__ void join(float &m, float &l, float *o, float m2, flo
 
 template <typename T, int LPR, int HEADS>
 __global__ void __launch_bounds__(32 * kStreamWarps)
-    attn_stream_kernel(const __grid_constant__ gdl_attention a, int splits, T *__restrict__ out, float *__restrict__ lse) {
+    attn_stream_kernel(const __grid_constant__ gdl_attention a, int splits, T *__restrict__ out, float *__restrict__ lse,
+                       T *__restrict__ rest) {
     constexpr int E = Lane16<T>::n, KEYS = 32 / LPR, ROW = LPR * E;
     __shared__ float part[kStreamWarps][HEADS][2 + ROW];  // m, l, o of each warp
     __shared__ float mine[HEADS][2 + ROW];                // of the CTA
@@ -227,7 +228,8 @@ __global__ void __launch_bounds__(32 * kStreamWarps)
 #pragma unroll
             for (int r = 1; r < kMaxSplits; ++r)
                 if (r < splits) join<1>(mm, ll, &oo, rm[r], rl[r], &rv[r]);
-            store1(out + (qi * a.heads + h0 + h) * a.dim + d, ll == 0.0f ? 0.0f : oo / ll);
+            const int64_t at = (qi * a.heads + h0 + h) * a.dim + d;
+            store_rest(out + at, rest ? rest + at : nullptr, ll == 0.0f ? 0.0f : oo / ll);
             if (lse && d == 0)
                 lse[(int64_t)(h0 + h) * a.n_query + qi] = ll == 0.0f ? neg_inf() : (mm + log2f(ll)) * kLn2;
         }
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(32 * kStreamWarps)
 }
 
 template <typename T, int LPR, int HEADS>
-int launch(const gdl_attention &a, int splits, T *out, float *lse, cudaStream_t st) {
+int launch(const gdl_attention &a, int splits, T *out, float *lse, T *rest, cudaStream_t st) {
     const int group = a.heads / a.kv_heads, chunks = (group + HEADS - 1) / HEADS;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(ragged_slots(a.n_query, a.num_clouds, 1) * splits), (unsigned)(a.kv_heads * chunks));
@@ -248,20 +250,20 @@ int launch(const gdl_attention &a, int splits, T *out, float *lse, cudaStream_t 
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    GDL_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_stream_kernel<T, LPR, HEADS>, a, splits, out, lse));
+    GDL_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_stream_kernel<T, LPR, HEADS>, a, splits, out, lse, rest));
     return GDL_OK;
 }
 
 template <typename T, int LPR>
-int by_heads(const gdl_attention &a, int splits, T *out, float *lse, cudaStream_t st) {
+int by_heads(const gdl_attention &a, int splits, T *out, float *lse, T *rest, cudaStream_t st) {
     const int group = a.heads / a.kv_heads;
-    if (group == 1) return launch<T, LPR, 1>(a, splits, out, lse, st);
-    if (group == 2) return launch<T, LPR, 2>(a, splits, out, lse, st);
-    return launch<T, LPR, 4>(a, splits, out, lse, st);
+    if (group == 1) return launch<T, LPR, 1>(a, splits, out, lse, rest, st);
+    if (group == 2) return launch<T, LPR, 2>(a, splits, out, lse, rest, st);
+    return launch<T, LPR, 4>(a, splits, out, lse, rest, st);
 }
 
 template <typename T>
-int stream_forward(const gdl_attention &a, T *out, float *lse, cudaStream_t st) {
+int stream_forward(const gdl_attention &a, T *out, float *lse, T *rest, cudaStream_t st) {
     // CTAs to a row: enough for two to an SM over the call, while each still has a step of keys for its warps
     const int group = a.heads / a.kv_heads, chunks = group <= 2 ? 1 : (group + 3) / 4;
     const int64_t side = a.left < 0 || a.right < 0 ? a.n_key : a.left + a.right + 1 + a.num_sinks;
@@ -269,11 +271,11 @@ int stream_forward(const gdl_attention &a, T *out, float *lse, cudaStream_t st) 
     int splits = 1;
     while (splits < kMaxSplits && ctas * splits * 2 <= 2 * kSmCount && span / (splits * 2) >= 64) splits *= 2;
     const int per = 16 / (int)sizeof(T);
-    if (a.dim <= 2 * per) return by_heads<T, 2>(a, splits, out, lse, st);
-    if (a.dim <= 4 * per) return by_heads<T, 4>(a, splits, out, lse, st);
-    if (a.dim <= 8 * per) return by_heads<T, 8>(a, splits, out, lse, st);
-    if (a.dim <= 16 * per) return by_heads<T, 16>(a, splits, out, lse, st);
-    return by_heads<T, 32>(a, splits, out, lse, st);
+    if (a.dim <= 2 * per) return by_heads<T, 2>(a, splits, out, lse, rest, st);
+    if (a.dim <= 4 * per) return by_heads<T, 4>(a, splits, out, lse, rest, st);
+    if (a.dim <= 8 * per) return by_heads<T, 8>(a, splits, out, lse, rest, st);
+    if (a.dim <= 16 * per) return by_heads<T, 16>(a, splits, out, lse, rest, st);
+    return by_heads<T, 32>(a, splits, out, lse, rest, st);
 }
 
 }  // namespace
@@ -291,9 +293,9 @@ bool takes_stream(const gdl_attention &a) {
            fits(a.q, a.q_head, a.q_row) && fits(a.k, a.k_head, a.k_row) && fits(a.v, a.v_head, a.v_row);
 }
 
-int attention_forward_stream(const gdl_attention &a, void *out, float *lse, cudaStream_t st) {
-    return a.dtype == GDL_DTYPE_F32 ? stream_forward<float>(a, (float *)out, lse, st)
-                                    : stream_forward<uint16_t>(a, (uint16_t *)out, lse, st);
+int attention_forward_stream(const gdl_attention &a, void *out, float *lse, void *rest, cudaStream_t st) {
+    return a.dtype == GDL_DTYPE_F32 ? stream_forward<float>(a, (float *)out, lse, nullptr, st)
+                                    : stream_forward<uint16_t>(a, (uint16_t *)out, lse, (uint16_t *)rest, st);
 }
 
 }  // namespace gdl

@@ -462,9 +462,9 @@ typedef struct {
 
 /* out [n_query, heads, dim] contiguous; lse [heads, n_query] f32 (nullable): natural logarithm of the
  * softmax denominators, which the backward needs. out_rest (nullable; shape and type of out, bf16 only):
- * what the rounding of out to bf16 left over (0 where a kernel does not compute it). The backward takes
- * delta = grad_out . out from both. It is worth little: dq is off by 0.00244 with it and by 0.00248 without
- * (16 x 2048 points, 4 heads of 32), by 0.00239 and 0.00240 at 131072 points, dbias by as much either way. */
+ * what the rounding of out to bf16 left over. The backward takes delta = grad_out . out from both, in effect
+ * from an output of 16 bits: dbias, a sum of differences against delta most of which cancels, is off by
+ * 0.0018 with it and by 0.0071 without (13645 points, 12 heads of 64 over 6, window 1401, 12 buckets). */
 int gdl_window_attention(const gdl_attention *a, void *out, float *lse, void *out_rest, void *stream);
 
 /* Gradients for grad_out, out [n_query, heads, dim] contiguous, lse and out_rest (nullable) of the forward.

@@ -264,3 +264,20 @@ def test_second_passes_over_odd_numbers_of_tiles(dim, heads, kv, lens, name):
         # beyond what row 0 reaches, and in the other cloud
         far = min(2 * window[0] + 1 if n in ("dk", "dv", "dq") else window[0] + 1, lens[0])
         assert torch.equal(got[n][far:], clean[n][far:]), n
+
+
+@pytest.mark.parametrize("dim,lens_q", [(32, None), (64, None), (96, None), (128, None), (20, None), (64, [12])])
+def test_the_bias_gradient_sums_to_what_it_should(dim, lens_q):
+    """With one bucket the gradient of the table is the sum of all dS, which is 0: what comes out is the error of delta
+    = dO . O against sum_j P dP, the same that a gradient of few buckets is left with after most of it cancels. In 16
+    bits of P and of O its parts are roundings of 2^-17 each, independent of one another: 8 standard deviations of
+    their sum, and of dP's and the exponents' in f32 (2^-20). With P or O in 8 bits it is 5 times as far and more."""
+    c = make(52, [128], 8, 8, dim, torch.bfloat16, lens_q=lens_q, buckets=1, bias_dt=torch.float32)
+    got = call(c, (-1, -1), 0)["dbias"][:, 0].cpu().double()
+    for h in range(8):
+        q, k, v, do = (c[n][:, h].cpu().double() for n in ("q", "k", "v", "dout"))
+        p = torch.softmax(q @ k.T / dim ** 0.5, 1)
+        o = p @ v
+        ds = p * (do @ v.T - (do * o).sum(1, keepdim=True))
+        var = (do ** 2 * 2.0 ** -32 * ((p ** 2) @ (v ** 2) + o ** 2)).sum() + (ds ** 2).sum() * 2.0 ** -40
+        assert abs(float(got[h])) <= 8 * float(var) ** 0.5, (h, float(got[h]), float(var) ** 0.5)
