@@ -4,14 +4,17 @@
 // loads tiles of 64 keys by TMA and issues the products; S = Q K^T goes to TMEM, the softmax threads read
 // their row, add the bias, mask, take the running maximum and the sum, and write P over S as the A operand
 // of O += P V. P is rounded to bf16 for that product, as the instruction takes two operands of one type; the sum is
-// of P before it. The output's error against 64 bits is then 0.0023, where its own rounding alone makes 0.0017.
+// of P before it. The output's error against 64 bits is then 0.0023, where its own rounding alone makes 0.0017. (P in two
+// parts, EXACT below, makes it 0.0017 in inference too, for 249 instead of 236 us over 8 ragged scenes and 484 instead
+// of 431 in the last case below: not taken there.)
 // Only the tiles that some query of the CTA sees are visited: first the sinks', then the span of the windows.
 //
 // With the bias the kernel is bound by the instructions of the softmax threads (distance, bucket, lookup,
 // exponent: 12.6 to a pair of rows in the inner step, 24 in all, at 62 % of the issue rate), not by products
 // (13 % of the tensor pipe) or memory: S goes by 32 columns in two buffers, which lets 4 CTAs share an SM. 131072
-// points, 4 heads of 64, window 513, 32 buckets: 366 us with the rest of the output, 339 without (the counters
-// are of an earlier build of that). 2 x 16384 rows, 16 heads of 128 over 4, causal window 1024, no bias: 398 us.
+// points, 4 heads of 64, window 513, 32 buckets: 331 us in inference (the counters are of an earlier build of that),
+// 377 in a training step (EXACT, and what rounding the output left over is kept). 2 x 16384 rows, 16 heads of 128 over 4,
+// causal window 1024, no bias: 399 us.
 #include "attention_mma.cuh"
 
 namespace gdl {
