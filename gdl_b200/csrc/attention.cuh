@@ -170,7 +170,8 @@ __device__ __noinline__ void attention_row(const gdl_attention &a, int h, int64_
     float m = neg_inf(), l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int part = 0; part < 2; ++part) {
         const int64_t from = part ? r.lo : 0, to = part ? r.hi : r.sinks;
-        for (int64_t j0 = from; j0 < to; j0 += 32) {
+        // (one NaN makes the sum and every output NaN for good: after a step that diverged all rows come here)
+        for (int64_t j0 = from; j0 < to && l == l; j0 += 32) {
             const int64_t j = j0 + lane;
             const float s = j < to ? logit2<T>(a, h, sq, qi, k0 + j) : neg_inf();
             const float mn = fmaxf(m, warp_max(s));
