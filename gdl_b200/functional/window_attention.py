@@ -63,7 +63,7 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, ptr_q: Tensor, *, ptr_k: O
                   constants (no gradient).
 
     status        int32 CUDA tensor of one element, zeroed by the caller: receives GDL_ERR_TIMEOUT (6) if a
-                  bounded wait of a kernel gave up, forward or backward (never observed; its rows are NaN).
+                  bounded wait of a kernel gave up, forward or backward (its rows are then NaN).
 
     A row that sees no key gives 0, and so does one whose logits are all -inf (a bias may hold -inf); both take no
     part in a gradient. What a row does not see never reaches its result; a NaN or an infinity in q, or in a key that

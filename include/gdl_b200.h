@@ -457,7 +457,7 @@ typedef struct {
     float inv_radius2;               /* finite, at least 0                                            */
     const float *pos_q, *pos_k;      /* [n_query, 3], [n_key, 3] f32; needed with a bias              */
     int32_t *status;                 /* nullable device word: GDL_ERR_TIMEOUT if a bounded wait of a
-                                        kernel gave up (never observed; its rows are then NaN)        */
+                                        kernel gave up (its rows are then NaN)                        */
 } gdl_attention;
 
 /* out [n_query, heads, dim] contiguous; lse [heads, n_query] f32 (nullable): natural logarithm of the
